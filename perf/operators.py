@@ -42,8 +42,9 @@ def _attn(name, heads, n_tree, width, n_past, max_seq, layout, kv):
 
 
 def _verify(name, vocab, n_tree, width, sampled, temperature, top_p):
-    c = dict(kind="verify", vocab=vocab, n_tree=n_tree, width=width, sampled=sampled, temperature=temperature,
-             top_p=top_p)
+    # the parameters as the single-precision numbers that a sampler's are
+    c = dict(kind="verify", vocab=vocab, n_tree=n_tree, width=width, sampled=sampled,
+             temperature=float(np.float32(temperature)), top_p=float(np.float32(top_p)))
     return dict(c, name=name) if name else c
 
 
