@@ -85,6 +85,15 @@ def hip_lib() -> C.CDLL:
                                           _f32p]),
         "tf_hip_attn_decode_noalloc": (C.c_int, [C.c_int, vp, vp, vp, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                                  C.c_int32, C.c_int32, vp, vp]),
+        "tf_hip_tree_masks": (C.c_int, [_i32p, C.c_int32, _u64p]),
+        "tf_hip_attn_tree_ws": (C.c_int64, [C.c_int32] * 5),
+        "tf_hip_attn_tree": (C.c_int, [C.c_int, C.c_int, vp, C.c_int64, vp, vp, vp, C.c_int32, C.c_int32, C.c_int32,
+                                       C.c_int32, C.c_int32, C.c_int32, C.c_int32, vp, C.c_int64, vp, C.c_size_t, vp]),
+        "tf_hip_verify_tree_ws": (C.c_int64, [C.c_int32, C.c_int32]),
+        "tf_hip_verify_tree": (C.c_int, [C.c_int, vp, C.c_int64, C.c_int32, vp, vp, C.c_int32, vp, C.c_int64, C.c_float,
+                                         C.c_float, vp, vp, vp, vp, vp, C.c_size_t, vp]),
+        "tf_hip_keep_path": (C.c_int, [C.c_int, C.c_int, vp, vp, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
+                                       C.c_int32, C.c_int32, vp, vp, vp]),
         "tf_hip_argmax": (C.c_int, [C.c_int, _f32p, C.c_int32, _i32p]),
         "tf_hip_read_stream": (C.c_int, [C.c_int, C.c_size_t, C.c_int32, _f64p, _f64p, _u32p]),
         "tf_hip_copy_stream": (C.c_int, [C.c_int, C.c_size_t, C.c_int32, _f64p, _f64p, _u32p]),
@@ -522,6 +531,15 @@ def attn_prefill(q: np.ndarray, k: np.ndarray, v: np.ndarray, device: int = 0) -
     _op(hip_lib().tf_hip_attn_prefill(device, _f(q), _f(k), _f(v), seq, n_heads, n_kv, hd, _f(out)),
         "tf_hip_attn_prefill")
     return out
+
+
+def tree_masks(parent) -> np.ndarray:
+    """The mask rows of tf_hip_attn_tree for a tree of drafted tokens given by its parents: each
+    node's own bit and its ancestors', [n][ceil(n / 64)] uint64 (host memory)."""
+    p = np.ascontiguousarray(parent, dtype=np.int32)
+    masks = np.zeros((len(p), (len(p) + 63) // 64), np.uint64)
+    _op(hip_lib().tf_hip_tree_masks(_i(p), len(p), masks.ctypes.data_as(_u64p)), "tf_hip_tree_masks")
+    return masks
 
 
 def argmax(x: np.ndarray, device: int = 0) -> int:

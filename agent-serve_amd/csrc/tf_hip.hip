@@ -7,6 +7,7 @@
 // replayed once per token with attention limited to the prompt, as attn_prefill
 // does) and the greedy loop (token = previous argmax, no host round trip).
 #include <algorithm>
+#include <cmath>
 #include <cstdio>
 #include <mutex>
 #include <cstdlib>
@@ -1846,6 +1847,150 @@ int tf_hip_attn_decode_noalloc(int device, const float* q, const float* k_cache,
     a.fixed_pos = n_pos - 1;
     a.fixed_start = 0;
     return launch_attn_decode(a, (hipStream_t)stream) == hipSuccess ? 0 : TF_HIP_EDEVICE;
+}
+
+// ---------------------------------------------------------------- trees of drafted tokens
+
+namespace {
+
+// Makes `device` current for a call and the caller's device current again at its end.
+struct DeviceScope {
+    int before = -1;
+    bool ok = false;
+    explicit DeviceScope(int device) {
+        if (hipGetDevice(&before) != hipSuccess) return;
+        ok = before == device || hipSetDevice(device) == hipSuccess;
+        if (before == device) before = -1;
+    }
+    ~DeviceScope() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+bool tree_shape_ok(int32_t n_tree, int32_t n_kv, int32_t hd, int32_t n_past) {
+    return n_tree >= 1 && n_tree <= kTreeMax && n_kv >= 1 && hd >= 8 && hd <= 256 && hd % 8 == 0 && n_past >= 0 &&
+           (int64_t)n_past + n_tree <= INT32_MAX;
+}
+
+bool cache_ok(int kv_type, const void* k, const void* v, int32_t n_tree, int32_t n_past, int32_t max_seq,
+              int32_t layout) {
+    return (kv_type == TF_HIP_TYPE_F32 || kv_type == TF_HIP_TYPE_F16) && k && v && aligned(k, 16) && aligned(v, 16) &&
+           (int64_t)n_past + n_tree <= max_seq && (layout == TF_HIP_KV_SEQ_MAJOR || layout == TF_HIP_KV_HEAD_MAJOR);
+}
+
+bool tree_heads_ok(int32_t n_heads, int32_t n_kv) { return n_heads >= 1 && n_heads <= 1024 && n_heads % n_kv == 0; }
+
+}  // namespace
+
+int tf_hip_tree_masks(const int32_t* parent, int32_t n_tree, uint64_t* masks) {
+    if (!parent || !masks || n_tree < 1 || n_tree > kTreeMax || parent[0] >= 0) return TF_HIP_EINVAL;
+    for (int i = 1; i < n_tree; ++i)
+        if (parent[i] < 0 || parent[i] >= i) return TF_HIP_EINVAL;
+    const int words = (n_tree + 63) / 64;
+    for (int i = 0; i < n_tree; ++i) {
+        for (int w = 0; w < words; ++w) masks[i * words + w] = i ? masks[parent[i] * words + w] : 0;
+        masks[i * words + i / 64] |= (uint64_t)1 << (i % 64);
+    }
+    return 0;
+}
+
+int64_t tf_hip_attn_tree_ws(int32_t n_tree, int32_t n_heads, int32_t n_kv, int32_t hd, int32_t n_past) {
+    if (!tree_shape_ok(n_tree, n_kv, hd, n_past) || !tree_heads_ok(n_heads, n_kv)) return TF_HIP_EINVAL;
+    return (int64_t)tree_attn_ws_bytes(n_tree, n_heads, n_kv, hd, n_past);
+}
+
+int tf_hip_attn_tree(int device, int kv_type, const float* q, int64_t ldq, const void* k_cache, const void* v_cache,
+                     const uint64_t* masks, int32_t n_tree, int32_t n_heads, int32_t n_kv, int32_t hd, int32_t n_past,
+                     int32_t max_seq, int32_t layout, float* out, int64_t ldo, void* ws, size_t ws_bytes,
+                     void* stream) {
+    if (!tree_shape_ok(n_tree, n_kv, hd, n_past) || !tree_heads_ok(n_heads, n_kv) ||
+        !cache_ok(kv_type, k_cache, v_cache, n_tree, n_past, max_seq, layout) || !q || !out || !masks ||
+        !aligned(q, 4) || !aligned(out, 4) || !aligned(masks, 8) || !aligned(ws, 16) ||
+        ldq < (int64_t)n_heads * hd || ldo < (int64_t)n_heads * hd)
+        return TF_HIP_EINVAL;
+    const size_t need = tree_attn_ws_bytes(n_tree, n_heads, n_kv, hd, n_past);
+    if (need && (!ws || ws_bytes < need)) return TF_HIP_ESCRATCH;
+    DeviceScope dev(device);
+    if (!dev.ok) return TF_HIP_EDEVICE;
+    TreeAttnArgs a{};
+    a.q = q;
+    a.ldq = ldq;
+    a.kc = k_cache;
+    a.vc = v_cache;
+    a.masks = masks;
+    a.out = out;
+    a.ldo = ldo;
+    a.kv_type = kv_type;
+    a.n_tree = n_tree;
+    a.H = n_heads;
+    a.G = n_kv;
+    a.hd = hd;
+    a.n_past = n_past;
+    a.max_seq = max_seq;
+    a.layout = layout;
+    return launch_tree_attn(a, ws, (hipStream_t)stream) == hipSuccess ? 0 : TF_HIP_EDEVICE;
+}
+
+int64_t tf_hip_verify_tree_ws(int32_t n_tree, int32_t n_vocab) {
+    if (n_tree < 1 || n_tree > kTreeMax || n_vocab < 1 || n_vocab > TF_HIP_VERIFY_MAX_VOCAB) return TF_HIP_EINVAL;
+    return (int64_t)verify_ws_bytes(n_tree, n_vocab);
+}
+
+int tf_hip_verify_tree(int device, const float* logits, int64_t ld_logits, int32_t n_vocab, const int32_t* tokens,
+                       const int32_t* parent, int32_t n_tree, const float* draft, int64_t ld_draft, float temperature,
+                       float top_p, const float* draws, int32_t* path, int32_t* result, float* probs, void* ws,
+                       size_t ws_bytes, void* stream) {
+    const int64_t need = tf_hip_verify_tree_ws(n_tree, n_vocab);
+    if (need < 0 || !logits || !tokens || !parent || !draws || !path || !result || !aligned(logits, 4) ||
+        !aligned(tokens, 4) || !aligned(parent, 4) || !aligned(draft, 4) || !aligned(draws, 4) || !aligned(path, 4) ||
+        !aligned(result, 4) || !aligned(probs, 4) || !aligned(ws, 16) || ld_logits < n_vocab ||
+        (draft && ld_draft < n_vocab) || !std::isfinite(temperature) || top_p != top_p)
+        return TF_HIP_EINVAL;
+    if (!ws || ws_bytes < (size_t)need) return TF_HIP_ESCRATCH;
+    DeviceScope dev(device);
+    if (!dev.ok) return TF_HIP_EDEVICE;
+    VerifyArgs a{};
+    a.logits = logits;
+    a.ld = ld_logits;
+    a.tokens = tokens;
+    a.parent = parent;
+    a.draft = draft;
+    a.ld_draft = ld_draft;
+    a.draws = draws;
+    a.path = path;
+    a.result = result;
+    a.probs = probs;
+    a.n_tree = n_tree;
+    a.vocab = n_vocab;
+    a.temperature = temperature;
+    a.top_p = top_p;
+    return launch_verify(a, ws, (hipStream_t)stream) == hipSuccess ? 0 : TF_HIP_EDEVICE;
+}
+
+int tf_hip_keep_path(int device, int kv_type, void* k_cache, void* v_cache, int32_t n_layer, int32_t n_kv, int32_t hd,
+                     int32_t n_past, int32_t n_tree, int32_t max_seq, int32_t layout, const int32_t* path,
+                     const int32_t* n_path, void* stream) {
+    if (!tree_shape_ok(n_tree, n_kv, hd, n_past) || n_kv > 1024 || n_layer < 1 || n_layer > 4096 ||
+        !cache_ok(kv_type, k_cache, v_cache, n_tree, n_past, max_seq, layout) || !path || !n_path ||
+        !aligned(path, 4) || !aligned(n_path, 4))
+        return TF_HIP_EINVAL;
+    DeviceScope dev(device);
+    if (!dev.ok) return TF_HIP_EDEVICE;
+    KeepArgs a{};
+    a.kc = k_cache;
+    a.vc = v_cache;
+    a.path = path;
+    a.n_path = n_path;
+    a.n_layer = n_layer;
+    a.G = n_kv;
+    a.row16 = hd * (kv_type == TF_HIP_TYPE_F32 ? 4 : 2) / 16;
+    a.n_past = n_past;
+    a.n_tree = n_tree;
+    a.max_seq = max_seq;
+    a.layout = layout;
+    return launch_keep_path(a, (hipStream_t)stream) == hipSuccess ? 0 : TF_HIP_EDEVICE;
 }
 
 int tf_hip_sample(tf_hip_ctx* c, float temperature, float top_p, float r, int32_t* token) {

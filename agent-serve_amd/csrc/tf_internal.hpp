@@ -332,6 +332,55 @@ hipError_t launch_step_split(const StepArgs& a, int n_wg, hipStream_t st);
 hipError_t launch_step_f16(const StepArgs& a, int n_wg, hipStream_t st);
 hipError_t launch_step_q6k(const StepArgs& a, int n_wg, hipStream_t st);
 
+// ---------------------------------------------------------------- trees of drafted tokens
+constexpr int kTreeMax = TF_HIP_TREE_MAX;
+
+// One layer's attention of a tree's queries over a cache (k_tree.hip).
+struct TreeAttnArgs {
+    const float* q;  // [n_tree] rows of ldq floats, [H][hd] each
+    int64_t ldq;
+    const void* kc;  // this layer's cache, kv_type elements
+    const void* vc;
+    const uint64_t* masks;  // [n_tree][mask_words]
+    float* out;             // rows of ldo floats
+    int64_t ldo;
+    int kv_type, n_tree, H, G, hd, n_past, max_seq, layout;
+    // set by launch_tree_attn
+    int mask_words, S;
+    float* part_o;   // [n_tree H][S][hd]
+    float* part_ml;  // [n_tree H][S][2]
+};
+size_t tree_attn_ws_bytes(int n_tree, int H, int G, int hd, int n_past);
+hipError_t launch_tree_attn(const TreeAttnArgs& a, void* ws, hipStream_t st);
+
+// The accepted nodes' rows of all layers moved to the front of the tree's (k_tree.hip).
+struct KeepArgs {
+    void* kc;  // [n_layer] caches
+    void* vc;
+    const int32_t* path;
+    const int32_t* n_path;
+    int n_layer, G, row16, n_past, n_tree, max_seq, layout;  // row16: 16-byte pieces of a kv head's row
+};
+hipError_t launch_keep_path(const KeepArgs& a, hipStream_t st);
+
+// A tree of drafted tokens against the target's distributions (k_verify.hip).
+struct VerifyArgs {
+    const float* logits;  // [n_tree] rows of ld floats
+    int64_t ld;
+    const int32_t* tokens;
+    const int32_t* parent;
+    const float* draft;  // [n_tree] rows of ld_draft floats, or nullptr
+    int64_t ld_draft;
+    const float* draws;
+    int32_t* path;
+    int32_t* result;
+    float* probs;  // or nullptr
+    int n_tree, vocab;
+    float temperature, top_p;
+};
+size_t verify_ws_bytes(int n_tree, int vocab);
+hipError_t launch_verify(const VerifyArgs& a, void* ws, hipStream_t st);
+
 // Launchers (k_*.hip).
 constexpr int kGemvMaxK = 9216;  // row length launch_gemv's prologue holds in registers (9 float4 a thread)
 hipError_t launch_gemv(const GemvArgs& a, int rows_per_wave, hipStream_t st);

@@ -271,6 +271,80 @@ int tf_hip_attn_decode_noalloc(int device, const float* q, const float* k_cache,
                                int32_t n_heads, int32_t n_kv, int32_t hd, int32_t n_pos, int32_t max_seq,
                                int32_t layout, float* out, void* stream);
 
+/* ---------------------------------------------------------------- trees of drafted tokens
+ * One step of speculative decoding over a device-resident cache. No counterpart in the
+ * reference: they are for loops that draft several tokens, run the model once over all of
+ * them and keep what it agrees with, with the same results as decoding them one by one
+ * (attn_decode, attention.cpp:55-80; sample_logits, sampler.cpp:15-52). A tree has n_tree
+ * nodes, at most TF_HIP_TREE_MAX; node 0 is the last token that is settled, and a node's
+ * parent comes before it. Node i's key and value rows are at cache position n_past + i.
+ *
+ * As tf_hip_attn_decode_noalloc: pointers are memory of `device` unless said otherwise, the
+ * work is enqueued on `stream` (a hipStream_t of that device; NULL for the null stream) and
+ * not waited for, and nothing is allocated, freed or synchronised; calls may be captured
+ * into a graph once one has been made on the device outside capture (it loads the code). The
+ * caller's current device is left as it was. Intermediate results live in the caller's workspace `ws` (16-byte aligned, ws_bytes >= what the _ws call says,
+ * else TF_HIP_ESCRATCH), which belongs to the call until its work is done: calls that may
+ * overlap, and graphs that may, take one each. Its contents need no initialisation. */
+#define TF_HIP_TREE_MAX 256
+
+/* Host only, no GPU: each node's own bit and its ancestors', from host parents (parent[0] < 0,
+ * 0 <= parent[i] < i, else TF_HIP_EINVAL): masks [n_tree][ceil(n_tree / 64)] words, bit j % 64
+ * of word j / 64 for node j. */
+int tf_hip_tree_masks(const int32_t* parent, int32_t n_tree, uint64_t* masks);
+
+/* Attention of the tree's queries for one layer: node i's query heads attend to every position
+ * below n_past and to the nodes that masks row i names (tf_hip_tree_masks' rows, or any others;
+ * bits past n_tree are not looked at). q is n_tree rows of ldq floats and out n_tree rows of
+ * ldo floats, each beginning with [n_heads][hd] (q already rotated); the caches are
+ * [max_seq][n_kv][hd] or [n_kv][max_seq][hd] by `layout`, 16-byte aligned, fp32 or fp16 by
+ * kv_type (TF_HIP_TYPE_F32 or _F16) and read only; positions past n_past + n_tree are not used.
+ * A row that sees no position is 0. What a node's rows hold, infinities and NaN too, does
+ * not reach the queries that do not see it; a query that sees one with either may be NaN.
+ * hd is a multiple of 8 up to 256, n_heads a multiple of n_kv up to 1024. One query
+ * (n_tree = 1) is decode attention. Sums and softmax are in fp32; products of fp32 numbers
+ * keep 22 bits of each. out must not overlap q. */
+int64_t tf_hip_attn_tree_ws(int32_t n_tree, int32_t n_heads, int32_t n_kv, int32_t hd, int32_t n_past);
+int tf_hip_attn_tree(int device, int kv_type, const float* q, int64_t ldq, const void* k_cache, const void* v_cache,
+                     const uint64_t* masks, int32_t n_tree, int32_t n_heads, int32_t n_kv, int32_t hd, int32_t n_past,
+                     int32_t max_seq, int32_t layout, float* out, int64_t ldo, void* ws, size_t ws_bytes,
+                     void* stream);
+
+/* Verification of the drafted tokens: logits row i (of ld_logits floats) is the target's
+ * prediction after node i, tokens[i] and parent[i] the node's token and parent (parent[0] is
+ * not looked at; a node whose parent does not come before it, or whose token is not below
+ * n_vocab, is never accepted). The target's distribution P_i is softmax(logits / temperature)
+ * cut to the nucleus of top_p as sample_logits cuts it, logits that compare equal in ascending
+ * index order; temperature <= 0 is all on the first maximum. From node 0 on, a node's children
+ * are tried in index order, child c against draws[c] (a uniform draw in [0, 1)):
+ *   draft NULL: the children are the drafter's choices; c is accepted with the probability P
+ *     gives its token, of what earlier rejected tokens leave;
+ *   draft: row i (of ld_draft floats) is the distribution that node i's children were sampled
+ *     from, each on its own; with R_0 = P, the k-th child's token x is accepted if
+ *     draws[c] draft[x] < R_k[x], else R_{k+1} = max(R_k - draft, 0) over its sum.
+ * The first accepted child is the next node. Where none is, result[1] is the next token, the
+ * first in index order at which the running sum of what is left exceeds draws[0] times its
+ * total (temperature <= 0: the first maximum). result[0] counts the path's nodes, node 0
+ * included; path [n_tree] holds them in order, then -1. probs (may be NULL) receives P of each
+ * node's token at its parent, 0 where there is no such, and at 0 P of the next token. Tokens and
+ * the next one are distributed as sample_logits' would be. A NaN logit counts as -inf; a row
+ * of -inf alone is uniform. n_vocab is at most TF_HIP_VERIFY_MAX_VOCAB, temperature finite. */
+#define TF_HIP_VERIFY_MAX_VOCAB (1 << 19)
+int64_t tf_hip_verify_tree_ws(int32_t n_tree, int32_t n_vocab);
+int tf_hip_verify_tree(int device, const float* logits, int64_t ld_logits, int32_t n_vocab, const int32_t* tokens,
+                       const int32_t* parent, int32_t n_tree, const float* draft, int64_t ld_draft, float temperature,
+                       float top_p, const float* draws, int32_t* path, int32_t* result, float* probs, void* ws,
+                       size_t ws_bytes, void* stream);
+
+/* Keeps the accepted nodes: in every layer's K and V cache (n_layer caches of n_kv max_seq hd
+ * elements one after the other, as tf_hip_create lays them out; kv_type and layout as above)
+ * the row of position n_past + path[i] moves to n_past + i for i < *n_path. The path's nodes
+ * ascend, as tf_hip_verify_tree writes them (path and result): at the first that does not, or is not below
+ * n_tree, the path ends. The other rows stay as they are. */
+int tf_hip_keep_path(int device, int kv_type, void* k_cache, void* v_cache, int32_t n_layer, int32_t n_kv, int32_t hd,
+                     int32_t n_past, int32_t n_tree, int32_t max_seq, int32_t layout, const int32_t* path,
+                     const int32_t* n_path, void* stream);
+
 /* attn_prefill (attention.cpp:82-111, attention.hpp:29-30): causal GQA attention of seq
  * positions over their own rows. q [seq][n_heads][hd], k and v [seq][n_kv][hd] (already
  * rotated), out [seq][n_heads][hd]; hd 32, 64 or 128, n_heads / n_kv at most 8. */
