@@ -43,7 +43,6 @@ namespace tfk {
 namespace {
 
 typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
-typedef float f4_t __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ f4_t mfma(b8_t a, b8_t b, f4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);

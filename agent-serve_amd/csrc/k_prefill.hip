@@ -37,9 +37,7 @@ namespace tfk {
 
 namespace {
 
-typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
-typedef float f4_t __attribute__((ext_vector_type(4)));
 
 // ---------------------------------------------------------------- operands in MFMA fragment order
 //
@@ -1504,27 +1502,6 @@ __global__ __launch_bounds__(kBlock) void k_pf_rope_store(float* qkv, int64_t ld
 // shared by the query heads of the kv head.
 
 constexpr int kAttnTile = 32;  // keys per tile record
-
-// Max and sum of v over lanes l, l ^ 16, l ^ 32, l ^ 48 (the 4 lanes of one query in the
-// MFMA layout) with gfx950's lane swaps, no LDS: a swap leaves each lane its own value in
-// one register and its partner's in the other, and every lane adds the lower lane's value
-// first, so the 4 lanes get the same bits.
-__device__ __forceinline__ float quad_max(float v) {
-    const uint32_t u = __float_as_uint(v);
-    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    const float m = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    const uint32_t w = __float_as_uint(m);
-    const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ float quad_sum(float v) {
-    const uint32_t u = __float_as_uint(v);
-    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    const float s = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    const uint32_t w = __float_as_uint(s);
-    const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
 
 // Tile record of head size HD: K fragments [16-key half][32-dim chunk][hi, lo][lane][8],
 // V^T fragments [16-dim tile][hi, lo][lane][8], then 2^-ek_j [32] and 2^-ev_j [32] (0 for

@@ -3,9 +3,26 @@
 // Node i of the tree has its key and value at cache position n_past + i. Its query sees every
 // position below n_past and, of the tree, the nodes whose bit its mask sets:
 //   s_j = q_i . k_j / sqrt(hd),   o_i = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),   m = max_j s_j
-// over the positions j that it sees; a row that sees none is zero. The positions are cut into
-// splits, each with its own m and l = sum_j e^(s_j - m); the merge adds them as
-// sum_s e^(m_s - M) o_s / sum_s e^(m_s - M) l_s.
+// over the positions j that it sees; a row that sees none is zero.
+//
+// The n_rep query heads of a kv head times the nodes are the rows of two matrix products over the
+// positions, S^T = K Q^T and O^T = V^T P^T, on v_mfma_f32_16x16x32_f16 with an online softmax
+// between. fp32 operands enter as fp16 pairs hi + lo (22 significant bits): x y = hi_x hi_y +
+// hi_x lo_y + lo_x hi_y, the rest being 2^-22 of the product; fp16 caches are operands as they
+// are, so only q and p are pairs. Numbers are scaled by powers of two, exactly taken out again:
+//   a query row by its largest element; a tile's keys by the tile's largest, its values likewise
+//   (both in [2^14, 2^15): fp16 pairs hold 22 bits down to 2^-18 of that, and 2^-40 of it below);
+//   a weight by 2^14, so that weights down to 2^-18 of the row's largest keep 22 bits.
+// The softmax's running reference is the score's maximum in units of log2, rounded up to a whole
+// number: rescaling by 2^(old - new) is exact, and it is needed only when the maximum passes one.
+//
+// A workgroup takes 16 QS WR rows of one kv head and one split of the positions, 32 WP positions
+// at a time, each 32 a record in LDS in fragment order: wave (wr, wp) runs rows of group wr over
+// record wp of every step, and the WP waves of a row group are merged at the end. Half of the
+// threads load, scale and store keys, half values, one step ahead of the products; loads are two
+// steps ahead. Splits are merged by k_tree_merge; one split writes the output itself.
+#include <algorithm>
+
 #include "dev_common.hpp"
 #include "tf_internal.hpp"
 
@@ -13,85 +30,504 @@ namespace tfk {
 namespace {
 
 constexpr float kLog2e = 1.44269504088896341f;
+constexpr int kRec = 32;  // positions of a record
+constexpr int kWeightExp = 14;
 
-template <class T>
-__device__ __forceinline__ float cache_value(const T* p) {
-    return (float)*p;
+// 2^e for e in [-126, 127]
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+// The power of two that takes amax into [2^14, 2^15); 126 for 0 (a tile of zeros, exact in any scale).
+__device__ __forceinline__ int scale_exp(float amax) {
+    const int e = amax > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(amax) : 126;
+    return min(max(e, -126), 126);
 }
 
-// Grid (row t H + h, split), 4 waves: wave w takes the split's positions w, w + 4, ...; a lane holds the
-// dims lane, lane + 64, ... of its query and of its wave's output.
-template <class T>
-__global__ __launch_bounds__(kBlock) void k_tree_attn(const TreeAttnArgs a) {
-    constexpr int kDims = 4;  // hd <= 256
-    __shared__ float mo[kWavesPerBlock][kDims * 64], ml[kWavesPerBlock][2];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int t = blockIdx.x / a.H, h = blockIdx.x % a.H, g = h / (a.H / a.G), s = blockIdx.y;
+// Where a V^T fragment's (dim, key group) entry lies among its 64: dims of one group in an order that
+// leaves 8 consecutive lanes on 8 different 16-byte banks, for the reader (dims 0..7 or 8..15) and for
+// writers that hold 1, 2, 4 or 8 consecutive dims each.
+__device__ __forceinline__ int v_entry(int dim, int dt, int kg) {
+    const int b3 = dim >> 3 & 1;
+    return 16 * kg + 8 * b3 + ((dim & 7) ^ b3 ^ (dt << 1 & 6));
+}
+
+template <class T, int HP, int WR, int WP, int QS, bool EXACT>
+__global__ __launch_bounds__(64 * WR * WP) void k_tree_attn(const TreeAttnArgs a) {
+    constexpr bool kPair = sizeof(T) == 4;
+    constexpr int NW = WR * WP, NC = HP / 32, NT = HP / 16;
+    constexpr int F = HP / WR;       // elements a thread loads per step
+    constexpr int DV = F / 8;        // dims of 8 values each
+    constexpr int kFrag = kPair ? 2048 : 1024;  // bytes of a fragment: hi, then lo
+    constexpr int kKeys = 2 * NC * kFrag, REC = kKeys + NT * kFrag;
+    constexpr int BN = kRec * WP;
+    constexpr int kBufs = 2;
+    static_assert(NW % 2 == 0 && F % 8 == 0, "half of the waves load keys, half values");
+    constexpr int kMergeWords = QS * (4 * NT + 2);
+    constexpr int kRecords = kBufs * WP * REC, kMerge = WR * (WP - 1) * 64 * kMergeWords * 4;
+    __shared__ __align__(16) unsigned char lds[kRecords > kMerge ? kRecords : kMerge];
+    __shared__ float amax[2][NW];
+    __shared__ uint32_t bad[3][WP];  // positions of a record with an infinity or NaN, by step mod 3
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wr = wave % WR, wp = wave / WR;
+    const int l16 = lane & 15, gq = lane >> 4;
+    const int hd = EXACT ? HP : a.hd, rep = a.H / a.G, rows = a.n_tree * rep;
+    // kv head fastest, then split, then row block: the row blocks of one span of keys are G S apart
+    const int g = blockIdx.x % a.G, split = blockIdx.x / a.G % a.S, blk = blockIdx.x / (a.G * a.S);
     const int end = a.n_past + a.n_tree;
-    const int p0 = (int)((int64_t)end * s / a.S), p1 = (int)((int64_t)end * (s + 1) / a.S);
-    const float* q = a.q + (int64_t)t * a.ldq + (int64_t)h * a.hd;
-    float qv[kDims], o[kDims];
+    const int units = (end + BN - 1) / BN, per = (units + a.S - 1) / a.S;
+    const int u0 = split * per, steps = min(units - u0, per);
+    const int64_t stride = a.layout == TF_HIP_KV_HEAD_MAJOR ? hd : (int64_t)a.G * hd;  // elements a position
+    const int64_t base = kv_offset(a.layout, a.G, a.max_seq, hd, g, 0);
+
+    // ---- loads
+    // Keys: a wave's unit is 16 positions x 32 dims of a fragment, lane = (position lane / 4, 8 dims from
+    // 8 (lane % 4)), which is entry 16 (lane % 4) + (position ^ 2 (lane % 4)). Values: a thread holds the
+    // 8 positions of a key group (4 kg + 0..3 and 16 + 4 kg + 0..3, as the weights lie in the lanes) of
+    // DV dims.
+    constexpr int kHalf = NW / 2;
+    const bool key_wave = wave < kHalf;
+    const int tv = tid - 64 * kHalf;  // value threads
+    const int v_d = DV * (tv % (HP / DV)), v_kg = tv / (HP / DV) % 4, v_rec = tv / (4 * (HP / DV));
+    const T* src = (const T*)(key_wave ? a.kc : a.vc) + base;
+    T reg[F];
+    auto load8 = [&](const T* p, bool ok, T* to) {  // 8 elements at a multiple of 8
+        if constexpr (kPair) {
+            const float4 x = ok ? gload_f4(p) : make_float4(0, 0, 0, 0), y = ok ? gload_f4(p + 4) : make_float4(0, 0, 0, 0);
+            to[0] = x.x; to[1] = x.y; to[2] = x.z; to[3] = x.w;
+            to[4] = y.x; to[5] = y.y; to[6] = y.z; to[7] = y.w;
+        } else {
+            const uint4 x = ok ? gload_u4(p) : make_uint4(0, 0, 0, 0);
+            __builtin_memcpy(to, &x, 16);
+        }
+    };
+    auto load = [&](int step) {
+        const int p = BN * (u0 + step);
+        if (key_wave) {
 #pragma unroll
-    for (int i = 0; i < kDims; ++i) {
-        qv[i] = lane + 64 * i < a.hd ? q[lane + 64 * i] : 0.0f;
-        o[i] = 0.0f;
+            for (int u = 0; u < F / 8; ++u) {
+                const int wu = wave * (F / 8) + u;  // (record, half, chunk)
+                const int c = wu % NC, pos = p + 16 * (wu / NC) + (lane >> 2), d = 32 * c + 8 * (lane & 3);
+                load8(src + (int64_t)min(pos, end - 1) * stride + d, EXACT || d < hd, reg + 8 * u);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int pos = min(p + kRec * v_rec + 4 * v_kg + (j < 4 ? j : 12 + j), end - 1);
+                const T* q = src + (int64_t)pos * stride + v_d;
+                T* to = reg + j * DV;
+                const bool ok = EXACT || v_d < hd;
+                if constexpr (DV == 8) {
+                    load8(q, ok, to);
+                } else if constexpr (DV * sizeof(T) == 16) {
+                    const uint4 x = ok ? gload_u4(q) : make_uint4(0, 0, 0, 0);
+                    __builtin_memcpy(to, &x, 16);
+                } else if constexpr (DV * sizeof(T) == 8) {
+                    const uint2 x = ok ? gload_u2(q) : make_uint2(0, 0);
+                    __builtin_memcpy(to, &x, 8);
+                } else if constexpr (DV * sizeof(T) == 4) {
+                    const uint32_t x = ok ? *(const TF_GLOBAL uint32_t*)q : 0u;
+                    __builtin_memcpy(to, &x, 4);
+                } else {
+                    to[0] = ok ? *gptr(q) : (T)0;
+                }
+            }
+        }
+    };
+    // the largest finite magnitude of this wave's elements, for their scale
+    auto publish = [&](int step) {
+        if constexpr (kPair) {
+            float m = 0.0f;
+#pragma unroll
+            for (int i = 0; i < F; ++i) m = fmaxf(m, fabsf((float)reg[i]));
+            if (!(m < INFINITY)) {
+                m = 0.0f;
+#pragma unroll
+                for (int i = 0; i < F; ++i) {
+                    const float x = fabsf((float)reg[i]);
+                    if (x < INFINITY) m = fmaxf(m, x);
+                }
+            }
+            m = wave_max(m);
+            if (lane == 0) amax[step & 1][wave] = m;
+        }
+    };
+    // The next step's scales. Values far below earlier ones are not scaled all the way up: their weights
+    // shrink by as much (they go into the same sum), and are to stay in range.
+    constexpr int kMostUp = 30;
+    int ek = 0, ev = 0, ev_min = 126 - kMostUp;
+    auto scales = [&](int step) {
+        if constexpr (kPair) {
+            float mk = 0.0f, mv = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kHalf; ++w) {
+                mk = fmaxf(mk, amax[step & 1][w]);
+                mv = fmaxf(mv, amax[step & 1][kHalf + w]);
+            }
+            ek = __builtin_amdgcn_readfirstlane(scale_exp(mk));
+            ev = min(__builtin_amdgcn_readfirstlane(scale_exp(mv)), ev_min + kMostUp);
+            ev_min = min(ev_min, ev);
+        }
+    };
+    auto put8 = [&](unsigned char* to, const T* x, float sc) {
+        h8_t hi;
+        if constexpr (kPair) {
+            h8_t lo;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float y = (float)x[j] * sc;
+                hi[j] = (_Float16)y;
+                lo[j] = (_Float16)(y - (float)hi[j]);
+            }
+            *(h8_t*)(to + 1024) = lo;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) hi[j] = x[j];
+        }
+        *(h8_t*)to = hi;
+    };
+    // The loaded step as records. A step that reaches into the tree takes its infinities and NaN out and
+    // notes their positions: a zero weight times one of them would be NaN in the rows that do not see it.
+    auto store = [&](int step) {
+        unsigned char* buf = lds + (step & 1) * WP * REC;
+        const bool tree = BN * (u0 + step + 1) > a.n_past;
+        const float sc = kPair ? pow2f(key_wave ? ek : ev) : 1.0f;
+        if (key_wave) {
+#pragma unroll
+            for (int u = 0; u < F / 8; ++u) {
+                const int wu = wave * (F / 8) + u, rec = wu / (2 * NC), hc = wu % (2 * NC);
+                if (tree) {
+                    bool fine = true;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const bool ok = fabsf((float)reg[8 * u + j]) < INFINITY;
+                        fine = fine && ok;
+                        reg[8 * u + j] = ok ? reg[8 * u + j] : (T)0;
+                    }
+                    if (!fine) atomicOr(&bad[step % 3][rec], 1u << (16 * (hc / NC) + (lane >> 2)));
+                }
+                const int ch = lane & 3;
+                put8(buf + rec * REC + hc * kFrag + 16 * (16 * ch + ((lane >> 2) ^ (2 * ch))), reg + 8 * u, sc);
+            }
+        } else {
+            if (tree) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    bool fine = true;
+#pragma unroll
+                    for (int i = 0; i < DV; ++i) {
+                        const bool ok = fabsf((float)reg[j * DV + i]) < INFINITY;
+                        fine = fine && ok;
+                        reg[j * DV + i] = ok ? reg[j * DV + i] : (T)0;
+                    }
+                    if (!fine) atomicOr(&bad[step % 3][v_rec], 1u << (4 * v_kg + (j < 4 ? j : 12 + j)));
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < DV; ++i) {
+                T x[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = reg[j * DV + i];
+                const int d = v_d + i, dt = d >> 4;
+                put8(buf + v_rec * REC + kKeys + dt * kFrag + 16 * v_entry(d & 15, dt, v_kg), x, sc);
+            }
+        }
+    };
+
+    if (tid < 3 * WP) bad[tid / WP][tid % WP] = 0;
+    load(0);
+
+    // ---- the wave's queries: lane l holds row l % 16 of each subtile, dims 32 c + 8 (l / 16) ..
+    h8_t qh[QS][NC], ql[QS][NC];
+    float fq[QS];
+    int row[QS];
+#pragma unroll
+    for (int qs = 0; qs < QS; ++qs) {
+        row[qs] = (blk * WR + wr) * 16 * QS + 16 * qs + l16;
+        const int r = min(row[qs], rows - 1);
+        const float* qr = a.q + (int64_t)(r / rep) * a.ldq + (int64_t)(g * rep + r % rep) * hd;
+        float v[NC][8], m = 0.0f;
+        const bool vec = (((uintptr_t)a.q | (uint64_t)a.ldq * 4) & 15) == 0;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int d = 32 * c + 8 * gq;
+            if (!EXACT && d >= hd) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[c][j] = 0.0f;
+            } else if (vec) {
+                const float4 x = gload_f4(qr + d), y = gload_f4(qr + d + 4);
+                v[c][0] = x.x; v[c][1] = x.y; v[c][2] = x.z; v[c][3] = x.w;
+                v[c][4] = y.x; v[c][5] = y.y; v[c][6] = y.z; v[c][7] = y.w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[c][j] = *gptr(qr + d + j);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[c][j]));
+        }
+        m = quad_max(m);
+        const int e = scale_exp(m);
+        const float sc = pow2f(e);
+        fq[qs] = ldexpf(kLog2e / sqrtf((float)hd), -e);  // scores in units of log2
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float x = v[c][j] * sc;
+                qh[qs][c][j] = (_Float16)x;
+                ql[qs][c][j] = (_Float16)(x - (float)qh[qs][c][j]);
+            }
     }
-    const float scale = kLog2e / sqrtf((float)a.hd);
-    float m = -INFINITY, l = 0.0f;
-    for (int p = p0 + wave; p < p1; p += kWavesPerBlock) {
-        const int j = p - a.n_past;
-        if (j >= 0 && !(a.masks[(int64_t)t * a.mask_words + (j >> 6)] >> (j & 63) & 1)) continue;
-        const int64_t at = kv_offset(a.layout, a.G, a.max_seq, a.hd, g, p);
-        const T *k = (const T*)a.kc + at, *v = (const T*)a.vc + at;
-        float x = 0.0f;
+    f4_t acc[QS][NT];  // O 2^(unit + 14)
+    float m_run[QS], l_run[QS];  // l of this lane's positions
+    int unit = 126;
 #pragma unroll
-        for (int i = 0; i < kDims; ++i)
-            if (lane + 64 * i < a.hd) x = fmaf(qv[i], cache_value(k + lane + 64 * i), x);
-        x = wave_sum(x) * scale;
-        const float m_new = x != x ? x : fmaxf(m, x);  // a NaN score stays in m or in l
-        const float alpha = m_new == m ? 1.0f : exp2f(m - m_new), w = x == m_new ? 1.0f : exp2f(x - m_new);
-        l = l * alpha + w;
-        m = m_new;
+    for (int qs = 0; qs < QS; ++qs) {
+        m_run[qs] = -INFINITY;
+        l_run[qs] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kDims; ++i)
-            if (lane + 64 * i < a.hd) o[i] = fmaf(w, cache_value(v + lane + 64 * i), o[i] * alpha);
+        for (int d = 0; d < NT; ++d) acc[qs][d] = (f4_t){0.0f, 0.0f, 0.0f, 0.0f};
     }
+    const int k_at = 16 * (16 * gq + (l16 ^ (2 * gq)));
+    int v_at[4];
 #pragma unroll
-    for (int i = 0; i < kDims; ++i) mo[wave][lane + 64 * i] = o[i];
-    if (lane == 0) {
-        ml[wave][0] = m;
-        ml[wave][1] = l;
+    for (int i = 0; i < 4; ++i) v_at[i] = 16 * v_entry(l16, i, gq);
+
+    // ---- one record: ke and ve its scales
+    auto record = [&](int step, int ke, int ve) {
+        const unsigned char* rec = lds + ((step & 1) * WP + wp) * REC;
+        const int p = BN * (u0 + step) + kRec * wp;
+        f4_t s[QS][2];
+#pragma unroll
+        for (int qs = 0; qs < QS; ++qs) s[qs][0] = s[qs][1] = (f4_t){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const unsigned char* f = rec + (half * NC + c) * kFrag + k_at;
+                const h8_t kh = *(const h8_t*)f;
+#pragma unroll
+                for (int qs = 0; qs < QS; ++qs) {
+                    s[qs][half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[qs][c], s[qs][half], 0, 0, 0);
+                    s[qs][half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[qs][c], s[qs][half], 0, 0, 0);
+                }
+                if constexpr (kPair) {
+                    const h8_t kl = *(const h8_t*)(f + 1024);
+#pragma unroll
+                    for (int qs = 0; qs < QS; ++qs)
+                        s[qs][half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[qs][c], s[qs][half], 0, 0, 0);
+                }
+            }
+        const bool tree = p + kRec > a.n_past;
+        uint32_t bits[QS], odd = 0;
+        if (tree) {
+            // bit b: the row sees position p + b
+            odd = bad[step % 3][wp];
+            const int off = p - a.n_past, left = end - p;
+#pragma unroll
+            for (int qs = 0; qs < QS; ++qs) {
+                const uint64_t* m = a.masks + (int64_t)(min(row[qs], rows - 1) / rep) * a.mask_words;
+                uint64_t x;
+                if (off < 0) {
+                    x = (m[0] << -off) | ((1ull << -off) - 1);
+                } else {
+                    const int w = off >> 6, sh = off & 63;
+                    x = m[w] >> sh;
+                    if (sh && w + 1 < a.mask_words) x |= m[w + 1] << (64 - sh);
+                }
+                bits[qs] = (uint32_t)x & (left >= 32 ? 0xFFFFFFFFu : (1u << left) - 1);
+            }
+        }
+        // values smaller than an earlier step's: the weights shrink; larger ones: the output does
+        int e = unit, shift = kWeightExp;
+        if constexpr (kPair) {
+            e = min(unit, ve);
+            shift = kWeightExp + e - ve;
+        } else {
+            e = 0;
+        }
+        const int de = e - unit;
+        unit = e;
+        h8_t ph[QS], pl[QS];
+        float resc[QS];
+        bool scaled = false;
+#pragma unroll
+        for (int qs = 0; qs < QS; ++qs) {
+            const float f = fmaxf(kPair ? ldexpf(fq[qs], -ke) : fq[qs], 1e-37f);
+            float x[8], mt = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = s[qs][j >> 2][j & 3];
+            if (tree) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int b = 4 * gq + (j < 4 ? j : 12 + j);
+                    if (odd >> b & 1) x[j] = NAN;
+                    if (!(bits[qs] >> b & 1)) x[j] = -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) mt = fmaxf(mt, x[j]);
+            mt = quad_max(mt);
+            const float m_new = fmaxf(m_run[qs], ceilf(mt * f));
+            const float m_ref = m_new == -INFINITY ? 0.0f : m_new;
+            const float alpha = __builtin_amdgcn_exp2f(m_run[qs] - m_ref);
+            const float sh = (float)shift - m_ref;
+            float ls = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float y = __builtin_amdgcn_exp2f(fmaf(x[j], f, sh));
+                ls += y;
+                ph[qs][j] = (_Float16)y;
+                pl[qs][j] = (_Float16)(y - (float)ph[qs][j]);
+            }
+            l_run[qs] = fmaf(l_run[qs], alpha, kPair ? ldexpf(ls, -shift) : ls * pow2f(-kWeightExp));
+            m_run[qs] = m_new;
+            resc[qs] = kPair ? ldexpf(alpha, de) : alpha;
+            scaled = scaled || resc[qs] != 1.0f;
+        }
+        if (__builtin_amdgcn_ballot_w64(scaled) != 0)
+#pragma unroll
+            for (int qs = 0; qs < QS; ++qs)
+#pragma unroll
+                for (int d = 0; d < NT; ++d) acc[qs][d] = acc[qs][d] * resc[qs];
+#pragma unroll
+        for (int d = 0; d < NT; ++d) {
+            const unsigned char* f = rec + kKeys + d * kFrag + v_at[d & 3];
+            const h8_t vh = *(const h8_t*)f;
+#pragma unroll
+            for (int qs = 0; qs < QS; ++qs) {
+                acc[qs][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[qs], acc[qs][d], 0, 0, 0);
+                acc[qs][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl[qs], acc[qs][d], 0, 0, 0);
+            }
+            if constexpr (kPair) {
+                const h8_t vl = *(const h8_t*)(f + 1024);
+#pragma unroll
+                for (int qs = 0; qs < QS; ++qs)
+                    acc[qs][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[qs], acc[qs][d], 0, 0, 0);
+            }
+        }
+    };
+
+    publish(0);
+    __syncthreads();
+    scales(0);
+    store(0);
+    int ke = ek, ve = ev;
+    if (steps > 1) {
+        load(1);
+        publish(1);
     }
     __syncthreads();
-    float M = -INFINITY, L = 0.0f, sum = 0.0f;
-    for (int w = 0; w < kWavesPerBlock; ++w) M = fmaxf(M, ml[w][0]);
-    for (int w = 0; w < kWavesPerBlock; ++w) {
-        const float f = ml[w][0] == -INFINITY ? 0.0f : exp2f(ml[w][0] - M);
-        L += f * ml[w][1];
-        if (f > 0.0f) sum = fmaf(f, mo[w][tid], sum);
+    // step t: records t are complete, and the loads of t + 1 with their scale
+    for (int t = 0; t < steps; ++t) {
+        if (t + 1 < steps) {
+            scales(t + 1);
+            store(t + 1);
+        }
+        if (tid < WP) bad[(t + 2) % 3][tid] = 0;
+        if (t + 2 < steps) load(t + 2);
+        if (BN * (u0 + t) + kRec * wp < end) record(t, ke, ve);
+        ke = ek;
+        ve = ev;
+        if (t + 2 < steps) publish(t + 2);
+        if (t + 1 < steps) __syncthreads();
     }
-    const int64_t part = (int64_t)blockIdx.x * a.S + s;
-    if (tid < a.hd) a.part_o[part * a.hd + tid] = sum;
-    if (tid == 0) {
-        a.part_ml[2 * part] = L == L ? M : L;
-        a.part_ml[2 * part + 1] = L;
+
+    // ---- the WP waves of a row group, then the row's 4 lanes
+#pragma unroll
+    for (int qs = 0; qs < QS; ++qs)
+        l_run[qs] = quad_sum(l_run[qs]);
+    if constexpr (WP > 1) {
+        float* mg = (float*)lds;  // [wp - 1][wr][word][lane]; unit is the same in all waves but in one without records
+        __syncthreads();
+        if (wp > 0) {
+            float* d = mg + (int64_t)((wp - 1) * WR + wr) * kMergeWords * 64 + lane;
+#pragma unroll
+            for (int qs = 0; qs < QS; ++qs) {
+#pragma unroll
+                for (int i = 0; i < 4 * NT; ++i) d[64 * (qs * (4 * NT + 2) + i)] = ldexpf(acc[qs][i >> 2][i & 3], -unit);
+                d[64 * (qs * (4 * NT + 2) + 4 * NT)] = m_run[qs];
+                d[64 * (qs * (4 * NT + 2) + 4 * NT + 1)] = l_run[qs];
+            }
+        }
+        __syncthreads();
+        if (wp > 0) return;
+#pragma unroll
+        for (int qs = 0; qs < QS; ++qs) {
+            float M = m_run[qs];
+            const float* b = mg + (int64_t)wr * kMergeWords * 64 + lane + 64 * qs * (4 * NT + 2);
+            constexpr int kNext = WR * kMergeWords * 64;
+#pragma unroll
+            for (int w = 0; w < WP - 1; ++w) M = fmaxf(M, b[w * kNext + 64 * 4 * NT]);
+            const float ref = M == -INFINITY ? 0.0f : M;
+            const float own = __builtin_amdgcn_exp2f(m_run[qs] - ref);
+            l_run[qs] *= own;
+#pragma unroll
+            for (int i = 0; i < 4 * NT; ++i) acc[qs][i >> 2][i & 3] = ldexpf(acc[qs][i >> 2][i & 3], -unit) * own;
+#pragma unroll
+            for (int w = 0; w < WP - 1; ++w) {
+                const float f = __builtin_amdgcn_exp2f(b[w * kNext + 64 * 4 * NT] - ref);
+                l_run[qs] = fmaf(f, b[w * kNext + 64 * (4 * NT + 1)], l_run[qs]);
+#pragma unroll
+                for (int i = 0; i < 4 * NT; ++i) acc[qs][i >> 2][i & 3] = fmaf(f, b[w * kNext + 64 * i], acc[qs][i >> 2][i & 3]);
+            }
+            m_run[qs] = M;
+        }
+    } else {
+#pragma unroll
+        for (int qs = 0; qs < QS; ++qs)
+#pragma unroll
+            for (int i = 0; i < 4 * NT; ++i) acc[qs][i >> 2][i & 3] = ldexpf(acc[qs][i >> 2][i & 3], -unit);
+    }
+#pragma unroll
+    for (int qs = 0; qs < QS; ++qs) {
+        if (row[qs] >= rows) continue;
+        const int t = row[qs] / rep, h = g * rep + row[qs] % rep;
+        if (a.S == 1) {
+            const float inv = l_run[qs] == 0.0f ? 0.0f : pow2f(-kWeightExp) / l_run[qs];
+            float* o = a.out + (int64_t)t * a.ldo + (int64_t)h * hd + 4 * gq;
+            const bool vec = (((uintptr_t)a.out | (uint64_t)a.ldo * 4) & 15) == 0;
+#pragma unroll
+            for (int d = 0; d < NT; ++d) {
+                if (!EXACT && 16 * d + 4 * gq >= hd) continue;
+                const f4_t x = acc[qs][d] * inv;
+                if (vec)
+                    *(f4_t*)(o + 16 * d) = x;
+                else
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[16 * d + i] = x[i];
+            }
+        } else {
+            const int64_t part = ((int64_t)t * a.H + h) * a.S + split;
+#pragma unroll
+            for (int d = 0; d < NT; ++d)
+                if (EXACT || 16 * d + 4 * gq < hd) *(f4_t*)(a.part_o + part * hd + 16 * d + 4 * gq) = acc[qs][d] * pow2f(-kWeightExp);
+            if (gq == 0) *(float2*)(a.part_ml + 2 * part) = make_float2(m_run[qs], l_run[qs]);
+        }
     }
 }
 
-// Merges the splits of row blockIdx.x.
+// Merges the splits: a thread per 4 dims of a row, o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.
 __global__ __launch_bounds__(kBlock) void k_tree_merge(const TreeAttnArgs a) {
-    const int t = blockIdx.x / a.H, h = blockIdx.x % a.H, d = threadIdx.x;
-    const int64_t part = (int64_t)blockIdx.x * a.S;
-    float M = -INFINITY, L = 0.0f, sum = 0.0f;
-    for (int s = 0; s < a.S; ++s) M = fmaxf(M, a.part_ml[2 * (part + s)]);
+    const int per = a.hd >> 2;
+    const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x, row = i / per;
+    if (row >= (int64_t)a.n_tree * a.H) return;
+    const int d = 4 * (int)(i % per);
+    const float* ml = a.part_ml + 2 * row * a.S;
+    const float* po = a.part_o + row * a.S * a.hd + d;
+    float M = -INFINITY;
+    for (int s = 0; s < a.S; ++s) M = fmaxf(M, ml[2 * s]);
+    if (M == -INFINITY) M = 0.0f;
+    float L = 0.0f;
+    f4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
     for (int s = 0; s < a.S; ++s) {
-        const float m = a.part_ml[2 * (part + s)];
-        if (m == -INFINITY) continue;
-        const float f = exp2f(m - M);
-        L = fmaf(f, a.part_ml[2 * (part + s) + 1], L);
-        if (d < a.hd) sum = fmaf(f, a.part_o[(part + s) * a.hd + d], sum);
+        const float f = __builtin_amdgcn_exp2f(ml[2 * s] - M);
+        L = fmaf(f, ml[2 * s + 1], L);
+        o += f * *(const f4_t*)(po + (int64_t)s * a.hd);
     }
-    if (d < a.hd) a.out[(int64_t)t * a.ldo + (int64_t)h * a.hd + d] = L == 0.0f ? 0.0f : sum / L;
+    o *= L == 0.0f ? 0.0f : 1.0f / L;
+    float* out = a.out + row / a.H * a.ldo + row % a.H * a.hd + d;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) out[k] = o[k];
 }
 
 // Row n_past + path[i] of every layer, K and V, moves to row n_past + i, for i up to the path's length or
@@ -118,29 +554,80 @@ __global__ __launch_bounds__(kBlock) void k_keep_path(const KeepArgs a) {
 
 }  // namespace
 
-int tree_attn_splits(int n_tree, int H, int G, int hd, int n_past) {
-    const int by_len = (n_past + n_tree + 63) / 64, by_rows = 2048 / (n_tree * H) + 1;
-    return by_len < by_rows ? by_len : by_rows;
+namespace {
+
+// Rows of a workgroup, positions of a step and splits for a call. See launch_tree_attn.
+struct TreePlan {
+    int hp, bm, bn, blocks, splits;
+};
+
+TreePlan tree_plan(int n_tree, int H, int G, int hd, int n_past) {
+    TreePlan p{};
+    const int rows = n_tree * (H / G);
+    p.hp = hd <= 64 ? 64 : (hd <= 128 ? 128 : 256);
+    if (p.hp == 256) {
+        p.bm = 64;
+        p.bn = 32;
+    } else if (p.hp == 128 && rows <= 32) {
+        p.bm = 32;
+        p.bn = 64;
+    } else if (p.hp == 64 && rows <= 16) {
+        p.bm = 16;
+        p.bn = 128;
+    } else {
+        p.bm = rows <= 64 ? 64 : 128;
+        p.bn = 64;
+    }
+    p.blocks = (rows + p.bm - 1) / p.bm;
+    const int64_t units = ((int64_t)n_past + n_tree + p.bn - 1) / p.bn;
+    const int64_t want = std::max<int64_t>(1, 256 / ((int64_t)G * p.blocks));
+    const int64_t per = (units + std::min(units, want) - 1) / std::min(units, want);
+    p.splits = (int)((units + per - 1) / per);
+    return p;
 }
 
+template <class T, int HP, int WR, int WP, int QS>
+hipError_t launch_tree(const TreeAttnArgs& a, const TreePlan& p, hipStream_t st) {
+    const dim3 grid((unsigned)(a.G * p.splits * p.blocks)), block(64 * WR * WP);
+    if (p.bm != 16 * QS * WR || p.bn != kRec * WP || p.hp != HP) return hipErrorInvalidValue;
+    if (a.hd == HP)
+        hipLaunchKernelGGL((k_tree_attn<T, HP, WR, WP, QS, true>), grid, block, 0, st, a);
+    else
+        hipLaunchKernelGGL((k_tree_attn<T, HP, WR, WP, QS, false>), grid, block, 0, st, a);
+    return hipGetLastError();
+}
+
+template <class T>
+hipError_t launch_tree_type(const TreeAttnArgs& a, const TreePlan& p, hipStream_t st) {
+    if (p.hp == 256) return launch_tree<T, 256, 4, 1, 1>(a, p, st);
+    if (p.hp == 128) {
+        if (p.bm == 32) return launch_tree<T, 128, 2, 2, 1>(a, p, st);
+        if (p.bm == 64) return launch_tree<T, 128, 4, 2, 1>(a, p, st);
+        return launch_tree<T, 128, 4, 2, 2>(a, p, st);
+    }
+    if (p.bm == 16) return launch_tree<T, 64, 1, 4, 1>(a, p, st);
+    if (p.bm == 64) return launch_tree<T, 64, 4, 2, 1>(a, p, st);
+    return launch_tree<T, 64, 4, 2, 2>(a, p, st);
+}
+
+}  // namespace
+
 size_t tree_attn_ws_bytes(int n_tree, int H, int G, int hd, int n_past) {
-    return (size_t)n_tree * H * tree_attn_splits(n_tree, H, G, hd, n_past) * (hd + 2) * 4;
+    const int S = tree_plan(n_tree, H, G, hd, n_past).splits;
+    return S == 1 ? 0 : (size_t)n_tree * H * S * (hd + 2) * 4;
 }
 
 hipError_t launch_tree_attn(const TreeAttnArgs& args, void* ws, hipStream_t st) {
     TreeAttnArgs a = args;
+    const TreePlan p = tree_plan(a.n_tree, a.H, a.G, a.hd, a.n_past);
     a.mask_words = (a.n_tree + 63) / 64;
-    a.S = tree_attn_splits(a.n_tree, a.H, a.G, a.hd, a.n_past);
+    a.S = p.splits;
     a.part_o = (float*)ws;
     a.part_ml = a.part_o + (size_t)a.n_tree * a.H * a.S * a.hd;
-    const dim3 grid((unsigned)(a.n_tree * a.H), (unsigned)a.S);
-    if (a.kv_type == TF_HIP_TYPE_F32)
-        hipLaunchKernelGGL(k_tree_attn<float>, grid, dim3(kBlock), 0, st, a);
-    else
-        hipLaunchKernelGGL(k_tree_attn<_Float16>, grid, dim3(kBlock), 0, st, a);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(k_tree_merge, dim3((unsigned)(a.n_tree * a.H)), dim3(kBlock), 0, st, a);
+    const hipError_t e = a.kv_type == TF_HIP_TYPE_F32 ? launch_tree_type<float>(a, p, st) : launch_tree_type<_Float16>(a, p, st);
+    if (e != hipSuccess || a.S == 1) return e;
+    const int64_t pieces = (int64_t)a.n_tree * a.H * (a.hd >> 2);
+    hipLaunchKernelGGL(k_tree_merge, dim3((unsigned)((pieces + kBlock - 1) / kBlock)), dim3(kBlock), 0, st, a);
     return hipGetLastError();
 }
 

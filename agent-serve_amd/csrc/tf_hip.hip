@@ -1871,7 +1871,7 @@ bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
 bool tree_shape_ok(int32_t n_tree, int32_t n_kv, int32_t hd, int32_t n_past) {
     return n_tree >= 1 && n_tree <= kTreeMax && n_kv >= 1 && hd >= 8 && hd <= 256 && hd % 8 == 0 && n_past >= 0 &&
-           (int64_t)n_past + n_tree <= INT32_MAX;
+           (int64_t)n_past + n_tree <= 1 << 30;
 }
 
 bool cache_ok(int kv_type, const void* k, const void* v, int32_t n_tree, int32_t n_past, int32_t max_seq,

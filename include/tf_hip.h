@@ -277,7 +277,8 @@ int tf_hip_attn_decode_noalloc(int device, const float* q, const float* k_cache,
  * them and keep what it agrees with, with the same results as decoding them one by one
  * (attn_decode, attention.cpp:55-80; sample_logits, sampler.cpp:15-52). A tree has n_tree
  * nodes, at most TF_HIP_TREE_MAX; node 0 is the last token that is settled, and a node's
- * parent comes before it. Node i's key and value rows are at cache position n_past + i.
+ * parent comes before it. Node i's key and value rows are at cache position n_past + i
+ * (n_past + n_tree at most 2^30).
  *
  * As tf_hip_attn_decode_noalloc: pointers are memory of `device` unless said otherwise, the
  * work is enqueued on `stream` (a hipStream_t of that device; NULL for the null stream) and
