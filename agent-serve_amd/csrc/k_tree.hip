@@ -505,24 +505,57 @@ __global__ __launch_bounds__(64 * WR * WP) void k_tree_attn(const TreeAttnArgs a
     }
 }
 
-// Merges the splits: a thread per 4 dims of a row, o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.
-__global__ __launch_bounds__(kBlock) void k_tree_merge(const TreeAttnArgs a) {
-    const int per = a.hd >> 2;
-    const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x, row = i / per;
-    if (row >= (int64_t)a.n_tree * a.H) return;
-    const int d = 4 * (int)(i % per);
-    const float* ml = a.part_ml + 2 * row * a.S;
-    const float* po = a.part_o + row * a.S * a.hd + d;
-    float M = -INFINITY;
-    for (int s = 0; s < a.S; ++s) M = fmaxf(M, ml[2 * s]);
-    if (M == -INFINITY) M = 0.0f;
-    float L = 0.0f;
+// Merges the splits: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s (the weights are powers of two).
+// tpr threads a row, in groups of hd / 4: a thread takes 4 dims of every (tpr / (hd / 4))-th split in one
+// round of loads, and the groups meet in LDS.
+__global__ __launch_bounds__(kBlock) void k_tree_merge(const TreeAttnArgs a, int tpr) {
+    __shared__ f4_t part[kBlock];
+    __shared__ float2 mls[kBlock];
+    const int per = a.hd >> 2, groups = tpr / per, in = threadIdx.x % tpr, grp = in / per, d = 4 * (in % per);
+    const int64_t row = (int64_t)blockIdx.x * (kBlock / tpr) + threadIdx.x / tpr;
+    const bool on = grp < groups && row < (int64_t)a.n_tree * a.H;
+    float M = -INFINITY, L = 0.0f;
     f4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 8
-    for (int s = 0; s < a.S; ++s) {
-        const float f = __builtin_amdgcn_exp2f(ml[2 * s] - M);
-        L = fmaf(f, ml[2 * s + 1], L);
-        o += f * *(const f4_t*)(po + (int64_t)s * a.hd);
+    if (on) {
+        const float2* ml = (const float2*)a.part_ml + row * a.S;
+        const float* po = a.part_o + row * a.S * a.hd + d;
+        constexpr int kRound = 8;
+        for (int s0 = grp; s0 < a.S; s0 += kRound * groups) {
+            float2 x[kRound];
+            f4_t y[kRound];
+#pragma unroll
+            for (int k = 0; k < kRound; ++k) {
+                const int s = min(s0 + k * groups, a.S - 1);
+                x[k] = ml[s];
+                y[k] = *(const f4_t*)(po + (int64_t)s * a.hd);
+            }
+            float top = M;
+#pragma unroll
+            for (int k = 0; k < kRound; ++k) top = fmaxf(top, x[k].x);
+            const float ref = top == -INFINITY ? 0.0f : top, f = __builtin_amdgcn_exp2f(M - ref);
+            L *= f;
+            o *= f;
+            M = top;
+#pragma unroll
+            for (int k = 0; k < kRound; ++k) {
+                if (s0 + k * groups >= a.S) continue;
+                const float w = __builtin_amdgcn_exp2f(x[k].x - ref);
+                L = fmaf(w, x[k].y, L);
+                o += w * y[k];
+            }
+        }
+    }
+    part[threadIdx.x] = o;
+    mls[threadIdx.x] = make_float2(M, L);
+    __syncthreads();
+    if (!on || grp) return;
+    for (int k = 1; k < groups; ++k) {
+        const float2 x = mls[threadIdx.x + k * per];
+        const float top = fmaxf(M, x.x), ref = top == -INFINITY ? 0.0f : top;
+        const float f = __builtin_amdgcn_exp2f(M - ref), w = __builtin_amdgcn_exp2f(x.x - ref);
+        L = fmaf(w, x.y, L * f);
+        o = o * f + w * part[threadIdx.x + k * per];
+        M = top;
     }
     o *= L == 0.0f ? 0.0f : 1.0f / L;
     float* out = a.out + row / a.H * a.ldo + row % a.H * a.hd + d;
@@ -565,19 +598,8 @@ TreePlan tree_plan(int n_tree, int H, int G, int hd, int n_past) {
     TreePlan p{};
     const int rows = n_tree * (H / G);
     p.hp = hd <= 64 ? 64 : (hd <= 128 ? 128 : 256);
-    if (p.hp == 256) {
-        p.bm = 64;
-        p.bn = 32;
-    } else if (p.hp == 128 && rows <= 32) {
-        p.bm = 32;
-        p.bn = 64;
-    } else if (p.hp == 64 && rows <= 16) {
-        p.bm = 16;
-        p.bn = 128;
-    } else {
-        p.bm = rows <= 64 ? 64 : 128;
-        p.bn = 64;
-    }
+    p.bn = kRec;
+    p.bm = p.hp == 256 || rows <= 64 ? 64 : (rows <= 256 ? 128 : 256);
     p.blocks = (rows + p.bm - 1) / p.bm;
     const int64_t units = ((int64_t)n_past + n_tree + p.bn - 1) / p.bn;
     const int64_t want = std::max<int64_t>(1, 256 / ((int64_t)G * p.blocks));
@@ -601,13 +623,13 @@ template <class T>
 hipError_t launch_tree_type(const TreeAttnArgs& a, const TreePlan& p, hipStream_t st) {
     if (p.hp == 256) return launch_tree<T, 256, 4, 1, 1>(a, p, st);
     if (p.hp == 128) {
-        if (p.bm == 32) return launch_tree<T, 128, 2, 2, 1>(a, p, st);
-        if (p.bm == 64) return launch_tree<T, 128, 4, 2, 1>(a, p, st);
-        return launch_tree<T, 128, 4, 2, 2>(a, p, st);
+        if (p.bm == 64) return launch_tree<T, 128, 4, 1, 1>(a, p, st);
+        if (p.bm == 128) return launch_tree<T, 128, 8, 1, 1>(a, p, st);
+        return launch_tree<T, 128, 8, 1, 2>(a, p, st);
     }
-    if (p.bm == 16) return launch_tree<T, 64, 1, 4, 1>(a, p, st);
-    if (p.bm == 64) return launch_tree<T, 64, 4, 2, 1>(a, p, st);
-    return launch_tree<T, 64, 4, 2, 2>(a, p, st);
+    if (p.bm == 64) return launch_tree<T, 64, 4, 1, 1>(a, p, st);
+    if (p.bm == 128) return launch_tree<T, 64, 8, 1, 1>(a, p, st);
+    return launch_tree<T, 64, 8, 1, 2>(a, p, st);
 }
 
 }  // namespace
@@ -626,8 +648,8 @@ hipError_t launch_tree_attn(const TreeAttnArgs& args, void* ws, hipStream_t st) 
     a.part_ml = a.part_o + (size_t)a.n_tree * a.H * a.S * a.hd;
     const hipError_t e = a.kv_type == TF_HIP_TYPE_F32 ? launch_tree_type<float>(a, p, st) : launch_tree_type<_Float16>(a, p, st);
     if (e != hipSuccess || a.S == 1) return e;
-    const int64_t pieces = (int64_t)a.n_tree * a.H * (a.hd >> 2);
-    hipLaunchKernelGGL(k_tree_merge, dim3((unsigned)((pieces + kBlock - 1) / kBlock)), dim3(kBlock), 0, st, a);
+    const int tpr = a.S <= 8 ? 64 : kBlock, rows = a.n_tree * a.H, per = kBlock / tpr;
+    hipLaunchKernelGGL(k_tree_merge, dim3((unsigned)((rows + per - 1) / per)), dim3(kBlock), 0, st, a, tpr);
     return hipGetLastError();
 }
 
