@@ -19,13 +19,18 @@
 // on one of up to half a million borders, so sums that are off by 2^-24 would move one draw in some
 // thousands. At 16 operations a logit that costs less than reading the logits does.
 //
-//   k_ver_chunks   a workgroup per row and 4096 logits: maximum, its index, sum of weights
-//   k_ver_nucleus  (instead, where top_p cuts) a workgroup per row: the kept tokens and their sum
-//   k_ver_rounds   (drafts with distributions) S_1 of the rows with two or more children
-//   k_ver_walk     one workgroup: every child's test at once, the path by its first accepted children,
-//                  and the draw where the chunks' sums serve it
-//   k_ver_draw     (else) the sums of what is left of the last row, and the draw by the workgroup that
-//                  ends last
+// Kernels, each with a workgroup per row and chunk of 4096 logits but for the walk:
+//   k_ver_chunks  a chunk's maximum, its index, minimum, sum of weights
+//   k_ver_bins    (where top_p cuts) the weights by 256 bins; the last workgroup of a row finds the bin
+//                 that the nucleus ends in
+//   k_ver_cut     (where top_p cuts) that bin's tokens in a list, the weights above it; the last workgroup
+//                 of a row finds the last token kept
+//   k_ver_rounds  (drafts with distributions) S_1 of the rows with two or more children
+//   k_ver_walk    every child's test at once, the path by its first accepted children, the draw. One
+//                 workgroup where the chunks' sums serve the draw; else one a chunk of the last row, all of
+//                 them walking for themselves, each summing what is left of its chunk, the last one drawing
+// "The last workgroup": every workgroup sends its part past the XCDs' caches (agent-scope stores), waits for
+// that, and counts itself; the one that counts all takes them in the same way. No workgroup waits for another.
 #include <climits>
 
 #include "dev_common.hpp"
@@ -39,36 +44,42 @@ constexpr int kVerThreads = 1024;
 constexpr int kVerWaves = kVerThreads / kWave;
 constexpr int kChunk = 4096;
 constexpr int kMaxChunks = (TF_HIP_VERIFY_MAX_VOCAB + kChunk - 1) / kChunk;
+constexpr int kBins = 256, kList = 4096, kFew = 256;
 constexpr double kLog2e64 = 1.4426950408889634;
 
 // Of one chunk of a row: its largest logit, that one's first index, and the weights' sum, the largest's 1.
 struct VerChunk {
     double sum;
-    float mx;
+    float mx, mn;  // mn: the least that is not -inf
     int32_t arg;
 };
 // One row's distribution: token x with logit l has probability w(l) / z where it is kept, that is
 // where its key is above thr, or equal to it with x <= cut; mx is the largest logit, first at arg.
 struct VerRow {
-    double z;
+    double z, inv_z;  // inv_z: 0 where nothing is kept
     float mx;
     uint32_t thr;
     int32_t cut;
     int32_t arg;
 };
-// What the draw takes from: row `at`, P without its children's tokens (drafts without distributions)
-// or max(P - t Q, 0).
-struct VerState {
-    double t;
-    int32_t at;
-    uint32_t arrived; // workgroups of k_ver_draw that have their sums
+// A row on the way to its nucleus: the bin of k_ver_bins that its end lies in, the mass above that bin, the
+// mass that the kept tokens reach, and the counts of workgroups that are done and of listed tokens.
+struct VerCut {
+    u64_t before, target;
+    float mx, mn;
+    int32_t bin;
+    uint32_t binned, listed, done;
 };
 struct VerWork {
-    VerState* state;
+    uint32_t* arrived;  // workgroups of k_ver_walk that have their sums
     VerRow* rows;       // [n]
+    VerCut* cuts;       // [n]
     VerChunk* chunks;   // [n][chunks a row]
     double* round;      // [n][chunks a row]: k_ver_rounds
-    u64_t* left;        // [chunks a row]: k_ver_draw's sums (doubles)
+    u64_t* mass;        // [n][chunks a row][kBins]
+    u64_t* above;       // [n][chunks a row]: doubles
+    u64_t* list;        // [n][kList]: logit, index
+    u64_t* left;        // [chunks a row]: k_ver_walk's sums (doubles)
     int n_chunks;
 };
 
@@ -103,7 +114,7 @@ __device__ __forceinline__ bool kept(const VerRow& r, float l, int x) {
     return k > r.thr || (k == r.thr && x <= r.cut);
 }
 __device__ __forceinline__ double prob(const VerRow& r, float l, int x, double c) {
-    return kept(r, l, x) && r.z > 0.0 ? weight(l, r.mx, c) / r.z : 0.0;
+    return kept(r, l, x) ? weight(l, r.mx, c) * r.inv_z : 0.0;
 }
 
 // Folds over the workgroup; every thread gets the result. red: a word for each wave.
@@ -181,260 +192,62 @@ constexpr int kChunkEach = kChunk / kBlock;
 __global__ __launch_bounds__(kBlock) void k_ver_chunks(const VerifyArgs a, const VerWork wk) {
     __shared__ u64_t red[kWavesPerBlock];
     const int row = blockIdx.y, x0 = blockIdx.x * kChunk, n = min(kChunk, a.vocab - x0);
-    if (row == 0 && blockIdx.x == 0 && threadIdx.x == 0) wk.state->arrived = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        if (row == 0) *wk.arrived = 0;
+        wk.cuts[row].binned = wk.cuts[row].listed = wk.cuts[row].done = 0;
+    }
     float v[kChunkEach];
     take<kChunkEach, false>(a.logits + (int64_t)row * a.ld + x0, n, NAN, v);
     u64_t best = 0;
+    float mn = INFINITY;
 #pragma unroll
     for (int k = 0; k < kChunkEach; ++k)
-        if (v[k] == v[k]) best = max(best, argmax_key(v[k], x0 + place<kChunkEach, false>(k)));
+        if (v[k] == v[k]) {
+            best = max(best, argmax_key(v[k], x0 + place<kChunkEach, false>(k)));
+            if (v[k] > -INFINITY) mn = fminf(mn, v[k]);
+        }
     best = block_max(best, red);
+    mn = block_fold(mn, red, [](float x, float y) { return fminf(x, y); });
     const int arg = best ? (int)(0xFFFFFFFFu - (uint32_t)best) : 0;
     const uint32_t key = (uint32_t)(best >> 32);
     const float mx = best ? __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key) : -INFINITY;
     double sum = 0.0;
-    if (a.temperature > 0.0f) {
+    if (a.temperature > 0.0f && !(a.top_p < 1.0f)) {
         const double c = kLog2e64 / (double)a.temperature;
 #pragma unroll
         for (int k = 0; k < kChunkEach; ++k) sum += weight(v[k], mx, c);
         sum = block_sum(sum, red);
     }
-    if (threadIdx.x == 0) wk.chunks[(int64_t)row * wk.n_chunks + blockIdx.x] = {sum, mx, arg};
+    if (threadIdx.x == 0) wk.chunks[(int64_t)row * wk.n_chunks + blockIdx.x] = {sum, mx, mn, arg};
 }
 
-// ---------------------------------------------------------------- the nucleus
-// The sums that find where it ends are of 32-bit weights (the last token's place is off only where the
-// running sum comes within 1e-7 of top_p), as integers of 2^-44 of the largest: integers add up to the
-// same in any order, so the atomics do not show. What is kept is summed in 64 bits.
-constexpr int kBins = 2048, kList = 2048;
-struct Nucleus {
-    u64_t mass[kBins];
-    uint2 list[kList];  // logit, index
-    u64_t red[kVerWaves];
-    u64_t before;       // the mass above the interval
-    uint32_t n_list, bin, k_lo, k_hi;
-};
-
-__device__ __forceinline__ u64_t weight_fix(float l, float mx, float c) {
-    const float w = l == mx ? 1.0f : __builtin_amdgcn_exp2f((l - mx) * c);
-    return (u64_t)(w * 17592186044416.0f);  // 2^44
-}
-
-// The bin whose masses reach `target` from s.before on; s.before grows by those above it.
-__device__ void find_bin(Nucleus& s, u64_t target) {
-    const int tid = threadIdx.x;
-    __syncthreads();
-    if (tid < 64) {
-        constexpr int kEach = kBins / 64;
-        u64_t sum = 0;
-        for (int i = 0; i < kEach; ++i) sum += s.mass[tid * kEach + i];
-        u64_t run = sum;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const u64_t up = __shfl_up(run, o);
-            if (tid >= o) run += up;
-        }
-        u64_t at = s.before + run - sum;
-        if (at < target && at + sum >= target) {
-            int b = tid * kEach;
-            while (at + s.mass[b] < target) at += s.mass[b++];
-            s.bin = b;
-            s.before = at;  // every lane of this wave has read it
-        }
-    }
-    __syncthreads();
-}
-
-// r.thr, r.cut and r.z of the tokens up to the one whose running sum reaches top_p. First the row's
-// logits in kBins bins of equal width below the maximum (as far as 24 temperatures, where a token's
-// weight is 2^-34 of the largest), then the elements of the bin that the sum ends in: few of them are
-// ranked directly; many are binned again by their keys, until few or one key is left.
-__device__ void nucleus(const float* p, int n, double c64, float top_p, float mn, VerRow& r, Nucleus& s) {
-    const int tid = threadIdx.x;
-    const float mx = r.mx, c = (float)c64;
-    const float span = fminf(mx - mn, 24.0f * (float)kLog2e64 / c);
-    const float inv = span > 0.0f && span < INFINITY ? (float)kBins / span : 0.0f;
-    auto bin_of = [&](float l) {
-        const float d = (mx - l) * inv;
-        return l == mx ? 0 : (d < (float)(kBins - 1) ? (int)d : kBins - 1);
-    };
-    for (int i = tid; i < kBins; i += kVerThreads) s.mass[i] = 0;
-    if (tid == 0) s.before = 0;
-    __syncthreads();
-    u64_t part = 0, low = 0;
-    each(p, n, [&](int, float l) {
-        if (!(l <= mx)) return;
-        const u64_t w = weight_fix(l, mx, c);
-        const int b = bin_of(l);
-        part += w;
-        if (b == kBins - 1)
-            low += w;
-        else
-            atomicAdd(&s.mass[b], w);
-    });
-    atomicAdd(&s.mass[kBins - 1], low);
-    const u64_t all = block_fold(part, s.red, [](u64_t a, u64_t b) { return a + b; });
-    top_p = fmaxf(top_p, 0.0f);
-    u64_t target = (u64_t)((double)top_p * (double)all);
-    // a token is kept while the sum before it is below top_p
-    if ((double)target < (double)top_p * (double)all) ++target;
-    target = target < 1 ? 1 : (target > all ? all : target);
-    find_bin(s, target);
-    const int b0 = s.bin;
-    uint32_t lo = 0, hi = 0xFFFFFFFFu;  // keys of the interval
-    auto inside = [&](float l) {
-        const uint32_t k = logit_key(l);
-        return l <= mx && bin_of(l) == b0 && k >= lo && k <= hi;
-    };
-    auto above = [&](float l) { return l <= mx && (bin_of(l) < b0 || (bin_of(l) == b0 && logit_key(l) > hi)); };
-    bool one_key = false;
-    double z = 0.0;
-    // the interval's elements, if they fit, and the weight above it
-    auto gather = [&]() {
-        __syncthreads();
-        if (tid == 0) s.n_list = 0;
-        __syncthreads();
-        z = 0.0;
-        each(p, n, [&](int x, float l) {
-            if (inside(l)) {
-                const uint32_t at = atomicAdd(&s.n_list, 1u);
-                if (at < kList) s.list[at] = make_uint2(__float_as_uint(l), (uint32_t)x);
-            }
-            if (above(l)) z += weight(l, mx, c64);
-        });
-        __syncthreads();
-        return s.n_list;
-    };
-    while (gather() > kList) {
-        __syncthreads();
-        if (tid == 0) {
-            s.k_lo = 0xFFFFFFFFu;
-            s.k_hi = 0;
-        }
-        for (int i = tid; i < kBins; i += kVerThreads) s.mass[i] = 0;
-        __syncthreads();
-        uint32_t a = 0xFFFFFFFFu, b = 0;
-        each(p, n, [&](int, float l) {
-            if (inside(l)) {
-                const uint32_t k = logit_key(l);
-                a = min(a, k);
-                b = max(b, k);
-            }
-        });
-        atomicMin(&s.k_lo, a);
-        atomicMax(&s.k_hi, b);
-        __syncthreads();
-        lo = s.k_lo;
-        hi = s.k_hi;
-        if (lo == hi) {  // one logit many times over
-            one_key = true;
-            break;
-        }
-        int shift = 0;
-        while (((hi - lo) >> shift) >= (uint32_t)kBins) ++shift;
-        each(p, n, [&](int, float l) {
-            if (inside(l)) atomicAdd(&s.mass[(hi - logit_key(l)) >> shift], weight_fix(l, mx, c));
-        });
-        find_bin(s, target);
-        const uint32_t top = hi - (s.bin << shift);
-        lo = max(lo, top - min(top, (1u << shift) - 1));
-        hi = top;
-    }
-    z = block_sum(z, s.red);
-    const u64_t before = s.before;
-    if (one_key) {
-        // the sum reaches the target at the k-th of them, in index order
-        const uint32_t bits = lo & 0x80000000u ? lo & 0x7FFFFFFFu : ~lo;
-        const float l1 = __uint_as_float(bits);
-        const u64_t w = weight_fix(l1, mx, c), k = (target - before + w - 1) / w;  // w > 0: the target lies here
-        int a = 0, b = n - 1;  // its index: halve the range by counts
-        while (a < b) {
-            const int mid = a + (b - a) / 2;
-            u64_t c0 = 0;
-            each(p, n, [&](int x, float l) { c0 += x <= mid && inside(l) ? 1 : 0; });
-            c0 = block_fold(c0, s.red, [](u64_t x, u64_t y) { return x + y; });
-            if (c0 >= k)
-                b = mid;
-            else
-                a = mid + 1;
-        }
-        r.thr = lo;
-        r.cut = a;
-        r.z = z + (double)k * weight(l1, mx, c64);
-        return;
-    }
-    const int m = (int)s.n_list;
-    for (int i = tid; i < m; i += kVerThreads) {
-        const float l = __uint_as_float(s.list[i].x);
-        const uint32_t k = logit_key(l), x = s.list[i].y;
-        u64_t sum = before;
-        for (int j = 0; j < m; ++j) {
-            const float lj = __uint_as_float(s.list[j].x);
-            const uint32_t kj = logit_key(lj);
-            if (kj > k || (kj == k && s.list[j].y < x)) sum += weight_fix(lj, mx, c);
-        }
-        if (sum < target && sum + weight_fix(l, mx, c) >= target) {
-            s.k_lo = k;
-            s.k_hi = x;
-        }
-    }
-    __syncthreads();
-    r.thr = s.k_lo;
-    r.cut = (int32_t)s.k_hi;
-    double in = 0.0;
-    for (int i = tid; i < m; i += kVerThreads) {
-        const float l = __uint_as_float(s.list[i].x);
-        if (kept(r, l, (int)s.list[i].y)) in += weight(l, mx, c64);
-    }
-    r.z = z + block_sum(in, s.red);
-}
-
-__global__ __launch_bounds__(kVerThreads) void k_ver_nucleus(const VerifyArgs a, const VerWork wk) {
-    __shared__ Nucleus s;
-    const int i = blockIdx.x, n = a.vocab;
-    const float* p = a.logits + (int64_t)i * a.ld;
-    if (i == 0 && threadIdx.x == 0) wk.state->arrived = 0;
-    u64_t best = 0;
-    float mn = INFINITY;
-    each(p, n, [&](int x, float l) {
-        if (l == l) {
-            best = max(best, argmax_key(l, x));
-            if (l > -INFINITY) mn = fminf(mn, l);
-        }
-    });
-    best = block_max(best, s.red);
-    mn = block_fold(mn, s.red, [](float x, float y) { return fminf(x, y); });
-    VerRow r;
-    r.arg = best ? (int32_t)(0xFFFFFFFFu - (uint32_t)best) : 0;
-    r.mx = best ? p[r.arg] : -INFINITY;
-    r.thr = 0;
-    r.cut = INT_MAX;
-    r.z = 0.0;
-    if (best) nucleus(p, n, kLog2e64 / (double)a.temperature, a.top_p, mn, r, s);
-    if (threadIdx.x == 0) wk.rows[i] = r;
-}
-
-// A row from its chunks, by one wave (every lane gets it).
+// A row from its chunks, by each 16 lanes of a wave that ask for one (all of them get it).
 __device__ __forceinline__ VerRow row_of_chunks(const VerifyArgs& a, const VerWork& wk, int row) {
-    const int lane = threadIdx.x & 63;
+    const int l16 = threadIdx.x & 15;
     const VerChunk* ch = wk.chunks + (int64_t)row * wk.n_chunks;
-    constexpr int kEach = (kMaxChunks + 63) / 64;
+    constexpr int kEach = kMaxChunks / 16;
+    static_assert(kMaxChunks % 16 == 0, "16 lanes take the chunks");
     VerChunk v[kEach];
     u64_t best = 0;
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
-        const bool on = lane + 64 * k < wk.n_chunks;
-        v[k] = on ? ch[lane + 64 * k] : VerChunk{0.0, -INFINITY, INT_MAX};
-        if (on) best = max(best, argmax_key(v[k].mx, v[k].arg));
+        if (16 * k >= wk.n_chunks) break;
+        v[k] = ch[min(l16 + 16 * k, wk.n_chunks - 1)];
     }
-    best = wave_max_u64(best);
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        if (16 * k >= wk.n_chunks) break;
+        best = max(best, argmax_key(v[k].mx, v[k].arg));
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) best = max(best, (u64_t)__shfl_xor(best, o));
     VerRow r;
     r.arg = (int32_t)(0xFFFFFFFFu - (uint32_t)best);
     const uint32_t key = (uint32_t)(best >> 32);
     r.mx = __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
     r.thr = 0;
     r.cut = INT_MAX;
-    r.z = 1.0;
+    r.z = r.inv_z = 1.0;
     if (a.temperature <= 0.0f) {
         r.thr = key;
         r.cut = r.arg;
@@ -442,11 +255,299 @@ __device__ __forceinline__ VerRow row_of_chunks(const VerifyArgs& a, const VerWo
         const double c = kLog2e64 / (double)a.temperature;
         double z = 0.0;
 #pragma unroll
-        for (int k = 0; k < kEach; ++k)
-            if (v[k].sum > 0.0) z += v[k].sum * weight(v[k].mx, r.mx, c);
-        r.z = wave_sum_d(z);
+        for (int k = 0; k < kEach; ++k) {
+            if (16 * k >= wk.n_chunks) break;
+            if (l16 + 16 * k < wk.n_chunks && v[k].sum > 0.0) z += v[k].sum * weight(v[k].mx, r.mx, c);
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) z += __shfl_xor(z, o);
+        r.z = z;
+        r.inv_z = z > 0.0 ? 1.0 / z : 0.0;
     }
     return r;
+}
+
+// The largest and the least logit of a row (but for -inf), from its chunks, in every thread.
+__device__ __forceinline__ void row_range(const VerWork& wk, int row, float& mx, float& mn) {
+    const int l64 = threadIdx.x & 63;
+    static_assert(kMaxChunks <= 128, "two chunks a lane");
+    const VerChunk* ch = wk.chunks + (int64_t)row * wk.n_chunks;
+    const int i0 = min(l64, wk.n_chunks - 1), i1 = min(l64 + 64, wk.n_chunks - 1);
+    mx = wave_max(fmaxf(ch[i0].mx, ch[i1].mx));
+    mn = -wave_max(-fminf(ch[i0].mn, ch[i1].mn));
+}
+
+// ---------------------------------------------------------------- the nucleus
+// The sums that find where it ends are of 32-bit weights (the last token's place is off only where the
+// running sum comes within 1e-7 of top_p), as integers of 2^-44 of the largest: integers add up to the
+// same in any order, so the atomics do not show. What is kept is summed in 64 bits.
+__device__ __forceinline__ u64_t weight_fix(float l, float mx, float c) {
+    const float w = l == mx ? 1.0f : __builtin_amdgcn_exp2f((l - mx) * c);
+    return (u64_t)(w * 17592186044416.0f);  // 2^44
+}
+// kBins bins of equal width below the maximum, as far as the least logit or 24 temperatures (where a token's
+// weight is 2^-34 of the largest); what is below is in the last one.
+struct Bins {
+    float mx, inv;
+    __device__ Bins(float mx, float mn, float c) : mx(mx) {
+        const float span = fminf(mx - mn, 24.0f * (float)kLog2e64 / c);
+        inv = span > 0.0f && span < INFINITY ? (float)kBins / span : 0.0f;
+    }
+    __device__ int operator()(float l) const {
+        const float d = (mx - l) * inv;
+        return l == mx ? 0 : (d < (float)(kBins - 1) ? (int)d : kBins - 1);
+    }
+};
+__device__ __forceinline__ void send(u64_t* p, u64_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ u64_t receive(const u64_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+// Counts this workgroup, whose parts every thread has sent; true in the last of n. sh: a word of LDS.
+__device__ __forceinline__ bool last_of(uint32_t* count, int n, int* sh) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) *sh = (int)__hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    return *sh == n - 1;
+}
+
+// The bin whose masses reach `target` from `before` on, for kBins = blockDim.x threads with a bin each; out: the
+// bin and the mass above it. red: a word for each wave.
+__device__ __forceinline__ void find_bin(u64_t mass, u64_t before, u64_t target, u64_t* red, int* out_bin, u64_t* out_before) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    u64_t run = mass;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const u64_t up = __shfl_up(run, o);
+        if (lane >= o) run += up;
+    }
+    __syncthreads();
+    if (lane == 63) red[wave] = run;
+    __syncthreads();
+    u64_t at = before + run - mass;
+    for (int i = 0; i < wave; ++i) at += red[i];
+    if (at < target && at + mass >= target) {
+        *out_bin = tid;
+        *out_before = at;
+    }
+    __syncthreads();
+}
+
+__global__ __launch_bounds__(kBlock) void k_ver_bins(const VerifyArgs a, const VerWork wk) {
+    __shared__ u64_t mass[kBins], red[kWavesPerBlock];
+    __shared__ u64_t sh_before;
+    __shared__ int sh, sh_bin;
+    static_assert(kBins == kBlock, "a bin a thread");
+    const int tid = threadIdx.x, row = blockIdx.y, x0 = blockIdx.x * kChunk, n = min(kChunk, a.vocab - x0);
+    float v[kChunkEach];
+    take<kChunkEach, false>(a.logits + (int64_t)row * a.ld + x0, n, NAN, v);
+    mass[tid] = 0;
+    float mx, mn;
+    row_range(wk, row, mx, mn);
+    __syncthreads();
+    const float c = (float)(kLog2e64 / (double)a.temperature);
+    const Bins bin(mx, mn, c);
+    u64_t low = 0;
+#pragma unroll
+    for (int k = 0; k < kChunkEach; ++k) {
+        if (!(v[k] <= mx)) continue;
+        const int b = bin(v[k]);
+        const u64_t w = weight_fix(v[k], mx, c);
+        if (b == kBins - 1)
+            low += w;
+        else
+            atomicAdd(&mass[b], w);
+    }
+    if (low) atomicAdd(&mass[kBins - 1], low);
+    __syncthreads();
+    u64_t* part = wk.mass + (int64_t)row * wk.n_chunks * kBins;
+    send(part + blockIdx.x * kBins + tid, mass[tid]);
+    VerCut& cut = wk.cuts[row];
+    if (!last_of(&cut.binned, wk.n_chunks, &sh)) return;
+    u64_t m = 0;
+#pragma unroll 8
+    for (int i = 0; i < wk.n_chunks; ++i) m += receive(part + i * kBins + tid);
+    const u64_t all = block_fold(m, red, [](u64_t x, u64_t y) { return x + y; });
+    const double want = (double)fmaxf(a.top_p, 0.0f) * (double)all;
+    u64_t target = (u64_t)want;
+    if ((double)target < want) ++target;  // a token is kept while the sum before it is below top_p
+    target = target < 1 ? 1 : (target > all ? all : target);
+    if (tid == 0) {
+        sh_bin = 0;
+        sh_before = 0;
+    }
+    find_bin(m, 0, target, red, &sh_bin, &sh_before);
+    if (tid == 0) {
+        cut.before = sh_before;
+        cut.target = target;
+        cut.mx = mx;
+        cut.mn = mn;
+        cut.bin = sh_bin;
+    }
+}
+
+// Which of a set of tokens the running sum ends at: `each` calls f(index, logit) for all of them (over the
+// workgroup's threads), `before` is the mass above them. Narrows their keys by bins until few are left, which
+// are ranked, or one logit many times over, of which the k-th in index order is the last.
+struct Settle {
+    u64_t mass[kBins], red[kWavesPerBlock];
+    uint2 few[kFew];
+    u64_t before;
+    uint32_t n, k_lo, k_hi;
+    int bin;
+};
+template <class Each>
+__device__ void settle(Each each_of, u64_t before, u64_t target, float mx, float c, Settle& s, uint32_t& thr, int32_t& cut) {
+    const int tid = threadIdx.x;
+    uint32_t lo = 0, hi = 0xFFFFFFFFu;
+    auto inside = [&](float l) {
+        const uint32_t k = logit_key(l);
+        return k >= lo && k <= hi;
+    };
+    for (;;) {
+        __syncthreads();
+        if (tid == 0) {
+            s.n = 0;
+            s.k_lo = 0xFFFFFFFFu;
+            s.k_hi = 0;
+            s.bin = 0;
+            s.before = before;
+        }
+        s.mass[tid] = 0;
+        __syncthreads();
+        uint32_t a = 0xFFFFFFFFu, b = 0;
+        each_of([&](int x, float l) {
+            if (!inside(l)) return;
+            const uint32_t k = logit_key(l), at = atomicAdd(&s.n, 1u);
+            if (at < kFew) s.few[at] = make_uint2(__float_as_uint(l), (uint32_t)x);
+            a = min(a, k);
+            b = max(b, k);
+        });
+        atomicMin(&s.k_lo, a);
+        atomicMax(&s.k_hi, b);
+        __syncthreads();
+        if (s.n <= kFew || s.k_lo == s.k_hi) break;
+        lo = s.k_lo;
+        hi = s.k_hi;
+        int shift = 0;
+        while (((hi - lo) >> shift) >= (uint32_t)kBins) ++shift;
+        each_of([&](int, float l) {
+            if (inside(l)) atomicAdd(&s.mass[(hi - logit_key(l)) >> shift], weight_fix(l, mx, c));
+        });
+        __syncthreads();
+        find_bin(s.mass[tid], before, target, s.red, &s.bin, &s.before);
+        before = s.before;
+        const uint32_t top = hi - ((uint32_t)s.bin << shift);
+        lo = max(lo, top - min(top, (1u << shift) - 1));
+        hi = top;
+    }
+    const int m = (int)s.n;
+    if (m > kFew) {
+        const uint32_t key = s.k_lo;
+        const float l1 = __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
+        const u64_t w = max(weight_fix(l1, mx, c), (u64_t)1), k = (target - before + w - 1) / w;
+        int a = 0, b = TF_HIP_VERIFY_MAX_VOCAB - 1;  // the least index with k of them up to it
+        while (a < b) {
+            const int mid = a + (b - a) / 2;
+            u64_t have = 0;
+            each_of([&](int x, float l) { have += x <= mid && logit_key(l) == key ? 1 : 0; });
+            have = block_fold(have, s.red, [](u64_t x, u64_t y) { return x + y; });
+            if (have >= k)
+                b = mid;
+            else
+                a = mid + 1;
+        }
+        thr = key;
+        cut = a;
+        return;
+    }
+    __syncthreads();
+    if (tid < m) {
+        const float l = __uint_as_float(s.few[tid].x);
+        const uint32_t k = logit_key(l), x = s.few[tid].y;
+        u64_t sum = before;
+        for (int j = 0; j < m; ++j) {
+            const float lj = __uint_as_float(s.few[j].x);
+            const uint32_t kj = logit_key(lj);
+            if (kj > k || (kj == k && s.few[j].y < x)) sum += weight_fix(lj, mx, c);
+        }
+        if (sum < target && sum + weight_fix(l, mx, c) >= target) {
+            s.k_lo = k;
+            s.k_hi = x;
+        }
+    }
+    __syncthreads();
+    thr = s.k_lo;
+    cut = (int32_t)s.k_hi;
+}
+
+__global__ __launch_bounds__(kBlock) void k_ver_cut(const VerifyArgs a, const VerWork wk) {
+    __shared__ uint2 list[kList];
+    __shared__ Settle s;
+    __shared__ uint32_t n_here, at_here;
+    __shared__ int sh;
+    const int tid = threadIdx.x, row = blockIdx.y, x0 = blockIdx.x * kChunk, n = min(kChunk, a.vocab - x0);
+    const float* p = a.logits + (int64_t)row * a.ld;
+    float v[kChunkEach];
+    take<kChunkEach, false>(p + x0, n, NAN, v);
+    VerCut& cut = wk.cuts[row];
+    const float mx = cut.mx;
+    const int b0 = cut.bin;
+    const double c64 = kLog2e64 / (double)a.temperature;
+    const float c = (float)c64;
+    const Bins bin(mx, cut.mn, c);
+    if (tid == 0) n_here = 0;
+    __syncthreads();
+    double above = 0.0;
+#pragma unroll
+    for (int k = 0; k < kChunkEach; ++k) {
+        const int b = v[k] <= mx ? bin(v[k]) : kBins;
+        if (b == b0) list[atomicAdd(&n_here, 1u)] = make_uint2(__float_as_uint(v[k]), (uint32_t)(x0 + place<kChunkEach, false>(k)));
+        if (b < b0) above += weight(v[k], mx, c64);
+    }
+    above = block_sum(above, s.red);
+    if (tid == 0) {
+        send(wk.above + (int64_t)row * wk.n_chunks + blockIdx.x, (u64_t)__double_as_longlong(above));
+        at_here = n_here ? __hip_atomic_fetch_add(&cut.listed, n_here, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+    }
+    __syncthreads();
+    for (uint32_t i = tid; i < n_here; i += kBlock)
+        if (at_here + i < kList) send(wk.list + (int64_t)row * kList + at_here + i, (u64_t)list[i].y << 32 | list[i].x);
+    if (!last_of(&cut.done, wk.n_chunks, &sh)) return;
+    const uint32_t m = __hip_atomic_load(&cut.listed, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    VerRow r;
+    r.mx = mx;
+    r.arg = 0;
+    r.thr = 0;
+    r.cut = INT_MAX;
+    double z = 0.0;
+    for (int i = tid; i < wk.n_chunks; i += kBlock) z += __longlong_as_double((long long)receive(wk.above + (int64_t)row * wk.n_chunks + i));
+    z = block_sum(z, s.red);
+    double in = 0.0;
+    auto settle_of = [&](auto each_of) {
+        settle(each_of, cut.before, cut.target, mx, c, s, r.thr, r.cut);
+        each_of([&](int x, float l) {
+            if (kept(r, l, x)) in += weight(l, mx, c64);
+        });
+    };
+    if (m <= kList) {
+        for (uint32_t i = tid; i < m; i += kBlock) {
+            const u64_t e = receive(wk.list + (int64_t)row * kList + i);
+            list[i] = make_uint2((uint32_t)e, (uint32_t)(e >> 32));
+        }
+        __syncthreads();
+        settle_of([&](auto f) {
+            for (uint32_t i = tid; i < m; i += kBlock) f((int)list[i].y, __uint_as_float(list[i].x));
+        });
+    } else {
+        // too many for the list (one logit thousands of times over, or a bin that most logits are in): from the row
+        settle_of([&](auto f) {
+            each(p, a.vocab, [&](int x, float l) {
+                if (l <= mx && bin(l) == b0) f(x, l);
+            });
+        });
+    }
+    r.z = z + block_sum(in, s.red);
+    r.inv_z = r.z > 0.0 ? 1.0 / r.z : 0.0;
+    if (tid == 0) wk.rows[row] = r;
 }
 
 // ---------------------------------------------------------------- sampled drafts: S_1
@@ -489,7 +590,7 @@ struct Left {
     __device__ double operator()(float lx, float qx, int x) const {
         if (!kept(r, lx, x)) return 0.0;
         const double w = weight(lx, r.mx, c);
-        if (q) return r.z > 0.0 ? fmax(w / r.z - t * (double)qx, 0.0) : 0.0;
+        if (q) return fmax(w * r.inv_z - t * (double)qx, 0.0);
         for (int i = 0; i < n_gone; ++i)
             if (gone[i] == x) return 0.0;
         return w;
@@ -515,19 +616,30 @@ template <int E>
 __device__ int draw(const Left& f, int vocab, const double* sums, int n_chunks, double u, u64_t* red, int* sh) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     __syncthreads();
-    double total = 0.0, before = 0.0;
-    for (int i = 0; i < n_chunks; ++i) total += sums[i];
-    if (!(total > 0.0)) return -1;
-    const double target = u * total;
-    int chunk = -1;
-    double run = 0.0;
-    for (int i = 0; i < n_chunks; ++i) {
-        if (sums[i] > 0.0 && (chunk < 0 || run <= target)) {  // up to the first that passes it, else the last
-            chunk = i;
-            before = run;
-        }
-        run += sums[i];
+    // every wave scans the chunks' sums: lane i holds those of 2 i and 2 i + 1
+    static_assert(kMaxChunks <= 128, "two chunks a lane");
+    const double s0 = 2 * lane < n_chunks ? sums[2 * lane] : 0.0, s1 = 2 * lane + 1 < n_chunks ? sums[2 * lane + 1] : 0.0;
+    double run = s0 + s1;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double x = __shfl_up(run, o);
+        if (lane >= o) run += x;
     }
+    const double total = __shfl(run, 63);
+    if (!(total > 0.0)) return -1;
+    const double target = u * total, b1 = run - s1;  // the sum up to the lane's second chunk
+    // the first chunk with anything left whose running sum passes the target, else the last with anything left
+    const u64_t over0 = __ballot(s0 > 0.0 && b1 > target), over1 = __ballot(s1 > 0.0 && run > target);
+    const u64_t any0 = __ballot(s0 > 0.0), any1 = __ballot(s1 > 0.0);
+    int chunk;
+    if (over0 | over1) {
+        const int i = __ffsll((unsigned long long)(over0 | over1)) - 1;
+        chunk = 2 * i + (over0 >> i & 1 ? 0 : 1);
+    } else {
+        const int i = 63 - __clzll(any0 | any1);
+        chunk = 2 * i + (any1 >> i & 1 ? 1 : 0);
+    }
+    const double before = __shfl(chunk & 1 ? b1 : b1 - s0, chunk >> 1);
     const int x0 = chunk * kChunk, n = min(kChunk, vocab - x0), at = E * tid;
     float l[E], q[E];
     double w[E], mine = 0.0;
@@ -581,16 +693,20 @@ __device__ __forceinline__ void put_next(const VerifyArgs& a, const VerRow& r, c
 }
 
 // ---------------------------------------------------------------- the walk
+constexpr int kWalkEach = kChunk / kVerThreads;
 __global__ __launch_bounds__(kVerThreads) void k_ver_walk(const VerifyArgs a, const VerWork wk) {
     __shared__ VerRow rows[kTreeMax];
-    __shared__ int parent[kTreeMax], token[kTreeMax], first[kTreeMax], gone[kTreeMax];
+    __shared__ __align__(16) int parent[kTreeMax];
+    __shared__ int token[kTreeMax], first[kTreeMax], gone[kTreeMax];
     __shared__ double pc[kTreeMax], qc[kTreeMax], draws[kTreeMax], s1[kTreeMax], sums[kMaxChunks];
     __shared__ u64_t red[kVerWaves];
     __shared__ int sh[4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.n_tree, V = a.vocab;
-    const bool greedy = a.temperature <= 0.0f, cut = !greedy && a.top_p < 1.0f;
+    const int tid = threadIdx.x, n = a.n_tree, V = a.vocab;
+    const bool greedy = a.temperature <= 0.0f, cut = !greedy && a.top_p < 1.0f, sampled = a.draft && !greedy;
+    const bool leader = blockIdx.x == 0;  // writes what all workgroups find alike
     const double c = greedy ? 0.0 : kLog2e64 / (double)a.temperature;
-    float lt = 0.0f, qt = 0.0f;
+    float lt = NAN, qt = 0.0f;
+    if (tid < kTreeMax) parent[tid] = -1;
     if (tid < n) {
         // a parent that does not come before its child, or a token that is none: never accepted
         int up = tid ? a.parent[tid] : -1;
@@ -600,56 +716,69 @@ __global__ __launch_bounds__(kVerThreads) void k_ver_walk(const VerifyArgs a, co
         token[tid] = x;
         first[tid] = INT_MAX;
         draws[tid] = (double)a.draws[tid];
-        const bool known = up >= 0 && x >= 0 && x < V;
-        lt = known ? a.logits[(int64_t)up * a.ld + x] : NAN;
-        qt = known && a.draft ? a.draft[(int64_t)up * a.ld_draft + x] : 0.0f;
+        if (up >= 0 && x >= 0 && x < V) {
+            lt = a.logits[(int64_t)up * a.ld + x];
+            if (sampled) qt = a.draft[(int64_t)up * a.ld_draft + x];
+        }
     }
-    for (int i = wave; i < n; i += kVerWaves) {
+    if (tid == 0) sh[2] = 0;
+    for (int i = tid >> 4; i < n; i += kVerThreads / 16) {
         const VerRow r = cut ? wk.rows[i] : row_of_chunks(a, wk, i);
-        if (lane == 0) rows[i] = r;
-        if (a.draft && !greedy) {
+        if ((tid & 15) == 0) rows[i] = r;
+        if (sampled) {
             double s = 0.0;
-            for (int k = lane; k < wk.n_chunks; k += 64) s += wk.round[(int64_t)i * wk.n_chunks + k];
-            s = wave_sum_d(s);
-            if (lane == 0) s1[i] = s;  // of rows with fewer than two children: not written, and not used
+            for (int k = tid & 15; k < wk.n_chunks; k += 16) s += wk.round[(int64_t)i * wk.n_chunks + k];
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o);
+            if ((tid & 15) == 0) s1[i] = s;  // of rows with fewer than two children: not written, and not used
         }
     }
     __syncthreads();
+    // the children's probabilities; of siblings with one token the first has it (drafts without distributions)
+    const int up = tid < n ? parent[tid] : -1;
+    uint32_t elder[kTreeMax / 32];  // elder siblings, a bit a node
+    int k = 0;
     if (tid < n) {
-        const int up = parent[tid], x = token[tid];
-        const double p = lt == lt && up >= 0 ? prob(rows[up], lt, x, c) : 0.0;
-        pc[tid] = p;
+        const double p = lt == lt && up >= 0 ? prob(rows[up], lt, token[tid], c) : 0.0;
+        bool again = false;
+#pragma unroll
+        for (int w = 0; w < kTreeMax / 32; ++w) {
+            elder[w] = 0;
+            if (32 * w >= tid || up < 0) continue;
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+                const int4 q = *(const int4*)&parent[32 * w + i];
+                elder[w] |= (uint32_t)(q.x == up) << i | (uint32_t)(q.y == up) << (i + 1) | (uint32_t)(q.z == up) << (i + 2) |
+                            (uint32_t)(q.w == up) << (i + 3);
+            }
+            if (tid < 32 * w + 32) elder[w] &= (1u << (tid - 32 * w)) - 1;
+            k += __popc(elder[w]);
+            for (uint32_t e = elder[w]; e; e &= e - 1) again |= token[32 * w + __ffs((int)e) - 1] == token[tid];
+        }
+        pc[tid] = sampled || !again ? p : 0.0;
         qc[tid] = (double)qt;
-        if (tid && a.probs) a.probs[tid] = (float)p;
+        if (tid && a.probs && leader) a.probs[tid] = (float)p;
     }
     __syncthreads();
     // every child's test, as if its parent were on the path and its elder siblings rejected
-    const bool sampled = a.draft && !greedy;
-    if (tid > 0 && tid < n && parent[tid] >= 0) {
-        const int up = parent[tid], x = token[tid];
-        int k = 0;
-        double before = 0.0, p = pc[tid];
-        for (int j = up + 1; j < tid; ++j) {
-            if (parent[j] != up) continue;
-            ++k;
-            if (sampled || greedy) continue;
-            bool again = false;  // a token counts once
-            for (int i = up + 1; i < j; ++i) again |= parent[i] == up && token[i] == token[j];
-            before += again ? 0.0 : pc[j];
-            if (token[j] == x) p = 0.0;
-        }
+    if (up >= 0) {
+        const double p = pc[tid];
         bool take = p > 0.0;
         if (sampled) {
-            const double t = k ? 1.0 : 0.0, left = p - t * qc[tid];
+            const double left = p - (k ? 1.0 : 0.0) * qc[tid];
             take = k < 2 && left > 0.0 && draws[tid] * qc[tid] * (k ? s1[up] : 1.0) < left;
         } else if (!greedy) {
+            double before = 0.0;
+#pragma unroll
+            for (int w = 0; w < kTreeMax / 32; ++w)
+                for (uint32_t e = elder[w]; e; e &= e - 1) before += pc[32 * w + __ffs((int)e) - 1];
             take = take && draws[tid] * (1.0 - before) < p;
         }
         if (take) atomicMin(&first[up], tid);
     }
     __syncthreads();
     int at = 0, count = 1;
-    if (tid == 0) a.path[0] = 0;
+    if (tid == 0 && leader) a.path[0] = 0;
     double t = 0.0;
     for (;;) {
         int next = first[at];
@@ -663,7 +792,7 @@ __global__ __launch_bounds__(kVerThreads) void k_ver_walk(const VerifyArgs a, co
                 if (kids >= 2) {
                     const Left f = {rows[at], a.logits + (int64_t)at * a.ld, a.draft + (int64_t)at * a.ld_draft, t, c, nullptr, 0};
                     S = 0.0;
-                    for (int ch = 0; ch < wk.n_chunks; ++ch) S += left_sum<kChunk / kVerThreads>(f, V, ch, red);
+                    for (int ch = 0; ch < wk.n_chunks; ++ch) S += left_sum<kWalkEach>(f, V, ch, red);
                     const double left = pc[j] - t * qc[j];
                     if (left > 0.0 && draws[j] * qc[j] * S < left) {
                         next = j;
@@ -676,98 +805,72 @@ __global__ __launch_bounds__(kVerThreads) void k_ver_walk(const VerifyArgs a, co
         }
         if (next == INT_MAX) break;
         at = next;
-        if (tid == 0) a.path[count] = at;
+        if (tid == 0 && leader) a.path[count] = at;
         ++count;
     }
-    for (int i = count + tid; i < n; i += kVerThreads) a.path[i] = -1;
     const VerRow r = rows[at];
     const float* l = a.logits + (int64_t)at * a.ld;
-    if (tid == 0) {
-        a.result[0] = count;
-        wk.state->at = at;
-        wk.state->t = t;
+    if (leader) {
+        for (int i = count + tid; i < n; i += kVerThreads) a.path[i] = -1;
+        if (tid == 0) a.result[0] = count;
     }
     if (greedy) {
         put_next(a, r, l, r.arg, c);
         return;
     }
-    if (cut || sampled) return;  // k_ver_draw
-    // the chunks' sums without the rejected tokens; a chunk that they were nearly all of is summed again
-    if (tid == 0) sh[2] = 0;
-    __syncthreads();
-    if (tid > at && tid < n && parent[tid] == at) gone[atomicAdd(&sh[2], 1)] = token[tid];
-    for (int i = tid; i < wk.n_chunks; i += kVerThreads) {
-        const VerChunk ch = wk.chunks[(int64_t)at * wk.n_chunks + i];
-        sums[i] = ch.sum > 0.0 ? ch.sum * weight(ch.mx, r.mx, c) : 0.0;
+    // the next token, from what is left of row `at`
+    if (!sampled && up == at) {
+        gone[k] = token[tid];
+        atomicMax(&sh[2], k + 1);
     }
     __syncthreads();
     const int n_gone = sh[2];
-    const Left f = {r, l, nullptr, 0.0, c, gone, n_gone};
-    for (int i = 0; i < n_gone; ++i) {
-        const int x = gone[i];
-        bool again = x < 0 || x >= V;
-        for (int k = 0; k < i; ++k) again |= gone[k] == x;
-        if (again) continue;
-        const int ch = x / kChunk;
-        const double w = weight(l[x], r.mx, c), old = sums[ch];
-        double now = old - w;
-        if (!(now > old * 0x1p-16)) now = left_sum<kChunk / kVerThreads>(f, V, ch, red);
-        __syncthreads();
-        if (tid == 0) sums[ch] = now;
-        __syncthreads();
-    }
-    int tok = draw<kChunk / kVerThreads>(f, V, sums, wk.n_chunks, draws[0], red, sh);
-    if (tok < 0) {  // nothing is left: from P itself
-        __syncthreads();
+    Left f = {r, l, sampled && t > 0.0 ? a.draft + (int64_t)at * a.ld_draft : nullptr, t, c, gone, n_gone};
+    auto chunk_sums = [&]() {  // P's own, from k_ver_chunks
         for (int i = tid; i < wk.n_chunks; i += kVerThreads) {
             const VerChunk ch = wk.chunks[(int64_t)at * wk.n_chunks + i];
             sums[i] = ch.sum > 0.0 ? ch.sum * weight(ch.mx, r.mx, c) : 0.0;
         }
-        const Left g = {r, l, nullptr, 0.0, c, gone, 0};
-        tok = draw<kChunk / kVerThreads>(g, V, sums, wk.n_chunks, draws[0], red, sh);
+        __syncthreads();
+    };
+    if (cut || sampled) {
+        const double mine = left_sum<kWalkEach>(f, V, blockIdx.x, red);
+        if (tid == 0) send(&wk.left[blockIdx.x], (u64_t)__double_as_longlong(mine));
+        if (!last_of(wk.arrived, wk.n_chunks, &sh[3])) return;
+        for (int i = tid; i < wk.n_chunks; i += kVerThreads) sums[i] = __longlong_as_double((long long)receive(&wk.left[i]));
+    } else {
+        // without the rejected tokens; a chunk that they were nearly all of is summed again
+        chunk_sums();
+        for (int i = 0; i < n_gone; ++i) {
+            const int x = gone[i];
+            bool again = x < 0 || x >= V;
+            for (int j = 0; j < i; ++j) again |= gone[j] == x;
+            if (again) continue;
+            const int ch = x / kChunk;
+            const double old = sums[ch];
+            double now = old - weight(l[x], r.mx, c);
+            if (!(now > old * 0x1p-16)) now = left_sum<kWalkEach>(f, V, ch, red);
+            __syncthreads();
+            if (tid == 0) sums[ch] = now;
+            __syncthreads();
+        }
     }
-    put_next(a, r, l, tok < 0 ? r.arg : tok, c);
-}
-
-// A workgroup per chunk of the last row; the one that ends last draws. Sums go out and come in past the
-// XCDs' caches (agent scope), each before its workgroup is counted.
-__global__ __launch_bounds__(kBlock) void k_ver_draw(const VerifyArgs a, const VerWork wk) {
-    __shared__ double sums[kMaxChunks];
-    __shared__ u64_t red[kWavesPerBlock];
-    __shared__ int gone[kTreeMax], sh[4];
-    const int tid = threadIdx.x;
-    const VerState st = *wk.state;
-    const double c = kLog2e64 / (double)a.temperature;
-    if (tid == 0) sh[2] = 0;
-    __syncthreads();
-    if (!a.draft && tid > st.at && tid < a.n_tree && a.parent[tid] == st.at) gone[atomicAdd(&sh[2], 1)] = a.tokens[tid];
-    const VerRow r = a.top_p < 1.0f ? wk.rows[st.at] : row_of_chunks(a, wk, st.at);
-    __syncthreads();
-    Left f = {r, a.logits + (int64_t)st.at * a.ld, a.draft && st.t > 0.0 ? a.draft + (int64_t)st.at * a.ld_draft : nullptr,
-              st.t, c, gone, sh[2]};
-    const double mine = left_sum<kChunkEach>(f, a.vocab, blockIdx.x, red);
-    if (tid == 0) {
-        __hip_atomic_store(&wk.left[blockIdx.x], (u64_t)__double_as_longlong(mine), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        sh[3] = (int)__hip_atomic_fetch_add(&wk.state->arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    __syncthreads();
-    if (sh[3] != wk.n_chunks - 1) return;
-    for (int i = tid; i < wk.n_chunks; i += kBlock)
-        sums[i] = __longlong_as_double((long long)__hip_atomic_load(&wk.left[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-    const double u = (double)a.draws[0];
-    int tok = draw<kChunkEach>(f, a.vocab, sums, wk.n_chunks, u, red, sh);
+    int tok = draw<kWalkEach>(f, V, sums, wk.n_chunks, draws[0], red, sh);
     if (tok < 0) {  // nothing is left: from P itself
         f.q = nullptr;
         f.n_gone = 0;
-        for (int ch = 0; ch < wk.n_chunks; ++ch) {
-            const double s = left_sum<kChunkEach>(f, a.vocab, ch, red);
-            __syncthreads();
-            if (tid == 0) sums[ch] = s;
+        __syncthreads();
+        if (cut) {
+            for (int ch = 0; ch < wk.n_chunks; ++ch) {
+                const double s = left_sum<kWalkEach>(f, V, ch, red);
+                if (tid == 0) sums[ch] = s;
+            }
+        } else {
+            chunk_sums();
         }
-        tok = draw<kChunkEach>(f, a.vocab, sums, wk.n_chunks, u, red, sh);
+        tok = draw<kWalkEach>(f, V, sums, wk.n_chunks, draws[0], red, sh);
     }
-    put_next(a, r, f.l, tok < 0 ? r.arg : tok, c);
+    put_next(a, r, l, tok < 0 ? r.arg : tok, c);
 }
 
 VerWork work_of(int n_tree, int vocab, void* ws, size_t* bytes) {
@@ -779,10 +882,15 @@ VerWork work_of(int n_tree, int vocab, void* ws, size_t* bytes) {
         p += (n + 63) / 64 * 64;
         return at;
     };
-    w.state = (VerState*)part(sizeof(VerState));
-    w.rows = (VerRow*)part((size_t)n_tree * sizeof(VerRow));
-    w.chunks = (VerChunk*)part((size_t)n_tree * w.n_chunks * sizeof(VerChunk));
-    w.round = (double*)part((size_t)n_tree * w.n_chunks * sizeof(double));
+    w.arrived = (uint32_t*)part(sizeof(uint32_t));
+    const size_t n = (size_t)n_tree, all = n * w.n_chunks;
+    w.rows = (VerRow*)part(n * sizeof(VerRow));
+    w.cuts = (VerCut*)part(n * sizeof(VerCut));
+    w.chunks = (VerChunk*)part(all * sizeof(VerChunk));
+    w.round = (double*)part(all * sizeof(double));
+    w.mass = (u64_t*)part(all * kBins * sizeof(u64_t));
+    w.above = (u64_t*)part(all * sizeof(u64_t));
+    w.list = (u64_t*)part(n * kList * sizeof(u64_t));
     w.left = (u64_t*)part((size_t)w.n_chunks * sizeof(u64_t));
     if (bytes) *bytes = (size_t)(p - (char*)ws);
     return w;
@@ -800,20 +908,16 @@ hipError_t launch_verify(const VerifyArgs& a, void* ws, hipStream_t st) {
     const VerWork wk = work_of(a.n_tree, a.vocab, ws, nullptr);
     const bool greedy = a.temperature <= 0.0f, cut = !greedy && a.top_p < 1.0f, sampled = !greedy && a.draft;
     const dim3 grid((unsigned)wk.n_chunks, (unsigned)a.n_tree);
-    hipError_t e;
-    if (cut)
-        hipLaunchKernelGGL(k_ver_nucleus, dim3((unsigned)a.n_tree), dim3(kVerThreads), 0, st, a, wk);
-    else
-        hipLaunchKernelGGL(k_ver_chunks, grid, dim3(kBlock), 0, st, a, wk);
-    if ((e = hipGetLastError()) != hipSuccess) return e;
-    if (sampled) {
-        hipLaunchKernelGGL(k_ver_rounds, grid, dim3(kBlock), 0, st, a, wk);
-        if ((e = hipGetLastError()) != hipSuccess) return e;
-    }
-    hipLaunchKernelGGL(k_ver_walk, dim3(1), dim3(kVerThreads), 0, st, a, wk);
-    if ((e = hipGetLastError()) != hipSuccess || !(cut || sampled)) return e;
-    hipLaunchKernelGGL(k_ver_draw, dim3((unsigned)wk.n_chunks), dim3(kBlock), 0, st, a, wk);
-    return hipGetLastError();
+    auto launch = [&](void (*k)(VerifyArgs, VerWork), dim3 g, int threads) {
+        hipLaunchKernelGGL(k, g, dim3(threads), 0, st, a, wk);
+        return hipGetLastError();
+    };
+    hipError_t e = launch(k_ver_chunks, grid, kBlock);
+    if (e == hipSuccess && cut) e = launch(k_ver_bins, grid, kBlock);
+    if (e == hipSuccess && cut) e = launch(k_ver_cut, grid, kBlock);
+    if (e == hipSuccess && sampled) e = launch(k_ver_rounds, grid, kBlock);
+    if (e == hipSuccess) e = launch(k_ver_walk, dim3(cut || sampled ? (unsigned)wk.n_chunks : 1u), kVerThreads);
+    return e;
 }
 
 }  // namespace tfk
