@@ -19,7 +19,7 @@
 // on one of up to half a million borders, so sums that are off by 2^-24 would move one draw in some
 // thousands. At 16 operations a logit that costs less than reading the logits does.
 //
-// Kernels, each with a workgroup per row and chunk of 4096 logits but for the walk:
+// Kernels, each with a workgroup per row and chunk of it (of 4096 or 8192 logits), but for the walk:
 //   k_ver_chunks  a chunk's maximum, its index, minimum, sum of weights
 //   k_ver_bins    (where top_p cuts) the weights by 256 bins; the last workgroup of a row finds the bin
 //                 that the nucleus ends in
@@ -44,7 +44,9 @@ constexpr int kVerThreads = 1024;
 constexpr int kVerWaves = kVerThreads / kWave;
 constexpr int kChunk = 4096;
 constexpr int kMaxChunks = (TF_HIP_VERIFY_MAX_VOCAB + kChunk - 1) / kChunk;
-constexpr int kBins = 256, kList = 4096, kFew = 256;
+// The nucleus' kernels: 16 logits a thread like the others, but half as many workgroups to count (a 64-node tree
+// over 128,256 logits: 256 threads 55.1 us a call, 512 54.2, 1024 60.8).
+constexpr int kCutThreads = 512, kCutChunk = 16 * kCutThreads, kBins = kCutThreads, kList = 4096, kFew = 256;
 constexpr double kLog2e64 = 1.4426950408889634;
 
 // Of one chunk of a row: its largest logit, that one's first index, and the weights' sum, the largest's 1.
@@ -54,11 +56,11 @@ struct VerChunk {
     int32_t arg;
 };
 // One row's distribution: token x with logit l has probability w(l) / z where it is kept, that is
-// where its key is above thr, or equal to it with x <= cut; mx is the largest logit, first at arg.
+// where l is above thr, or equal to it with x <= cut (-inf and INT_MAX: all but NaN); mx is the largest logit, first at arg.
 struct VerRow {
     double z, inv_z;  // inv_z: 0 where nothing is kept
     float mx;
-    uint32_t thr;
+    float thr;
     int32_t cut;
     int32_t arg;
 };
@@ -76,11 +78,11 @@ struct VerWork {
     VerCut* cuts;       // [n]
     VerChunk* chunks;   // [n][chunks a row]
     double* round;      // [n][chunks a row]: k_ver_rounds
-    u64_t* mass;        // [n][chunks a row][kBins]
-    u64_t* above;       // [n][chunks a row]: doubles
+    u64_t* mass;        // [n][kCutChunk chunks a row][kBins]
+    u64_t* above;       // [n][kCutChunk chunks a row]: doubles
     u64_t* list;        // [n][kList]: logit, index
     u64_t* left;        // [chunks a row]: k_ver_walk's sums (doubles)
-    int n_chunks;
+    int n_chunks, n_cuts;  // of a row, of kChunk and of kCutChunk logits
 };
 
 __device__ __forceinline__ uint32_t logit_key(float l) { return (uint32_t)(argmax_key(l, 0) >> 32); }
@@ -109,10 +111,7 @@ __device__ __forceinline__ double weight(float l, float mx, double c) {
     const double w = exp2_64(((double)l - (double)mx) * c);
     return l == mx ? 1.0 : w;
 }
-__device__ __forceinline__ bool kept(const VerRow& r, float l, int x) {
-    const uint32_t k = logit_key(l);
-    return k > r.thr || (k == r.thr && x <= r.cut);
-}
+__device__ __forceinline__ bool kept(const VerRow& r, float l, int x) { return l > r.thr || (l == r.thr && x <= r.cut); }
 __device__ __forceinline__ double prob(const VerRow& r, float l, int x, double c) {
     return kept(r, l, x) ? weight(l, r.mx, c) * r.inv_z : 0.0;
 }
@@ -167,7 +166,7 @@ __device__ __forceinline__ void each(const float* p, int n, F f) {
 template <int E, bool RUN>
 __device__ __forceinline__ int place(int k) {
     const int tid = (int)threadIdx.x;
-    return RUN ? E * tid + k : 4 * (tid + k / 4 * (kChunk / E)) + k % 4;
+    return RUN ? E * tid + k : 4 * (tid + k / 4 * (int)blockDim.x) + k % 4;
 }
 template <int E, bool RUN>
 __device__ __forceinline__ void take(const float* p, int n, float none, float* v) {
@@ -245,11 +244,11 @@ __device__ __forceinline__ VerRow row_of_chunks(const VerifyArgs& a, const VerWo
     r.arg = (int32_t)(0xFFFFFFFFu - (uint32_t)best);
     const uint32_t key = (uint32_t)(best >> 32);
     r.mx = __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
-    r.thr = 0;
+    r.thr = -INFINITY;
     r.cut = INT_MAX;
     r.z = r.inv_z = 1.0;
     if (a.temperature <= 0.0f) {
-        r.thr = key;
+        r.thr = r.mx;
         r.cut = r.arg;
     } else {
         const double c = kLog2e64 / (double)a.temperature;
@@ -331,14 +330,15 @@ __device__ __forceinline__ void find_bin(u64_t mass, u64_t before, u64_t target,
     __syncthreads();
 }
 
-__global__ __launch_bounds__(kBlock) void k_ver_bins(const VerifyArgs a, const VerWork wk) {
-    __shared__ u64_t mass[kBins], red[kWavesPerBlock];
+constexpr int kCutEach = kCutChunk / kCutThreads;
+__global__ __launch_bounds__(kCutThreads) void k_ver_bins(const VerifyArgs a, const VerWork wk) {
+    __shared__ u64_t mass[kBins], red[(kCutThreads / kWave)];
     __shared__ u64_t sh_before;
     __shared__ int sh, sh_bin;
-    static_assert(kBins == kBlock, "a bin a thread");
-    const int tid = threadIdx.x, row = blockIdx.y, x0 = blockIdx.x * kChunk, n = min(kChunk, a.vocab - x0);
-    float v[kChunkEach];
-    take<kChunkEach, false>(a.logits + (int64_t)row * a.ld + x0, n, NAN, v);
+    static_assert(kBins == kCutThreads, "a bin a thread");
+    const int tid = threadIdx.x, row = blockIdx.y, x0 = blockIdx.x * kCutChunk, n = min(kCutChunk, a.vocab - x0);
+    float v[kCutEach];
+    take<kCutEach, false>(a.logits + (int64_t)row * a.ld + x0, n, NAN, v);
     mass[tid] = 0;
     float mx, mn;
     row_range(wk, row, mx, mn);
@@ -347,7 +347,7 @@ __global__ __launch_bounds__(kBlock) void k_ver_bins(const VerifyArgs a, const V
     const Bins bin(mx, mn, c);
     u64_t low = 0;
 #pragma unroll
-    for (int k = 0; k < kChunkEach; ++k) {
+    for (int k = 0; k < kCutEach; ++k) {
         if (!(v[k] <= mx)) continue;
         const int b = bin(v[k]);
         const u64_t w = weight_fix(v[k], mx, c);
@@ -356,15 +356,23 @@ __global__ __launch_bounds__(kBlock) void k_ver_bins(const VerifyArgs a, const V
         else
             atomicAdd(&mass[b], w);
     }
-    if (low) atomicAdd(&mass[kBins - 1], low);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) low += __shfl_xor(low, o);
+    if ((tid & 63) == 0 && low) atomicAdd(&mass[kBins - 1], low);
     __syncthreads();
-    u64_t* part = wk.mass + (int64_t)row * wk.n_chunks * kBins;
+    u64_t* part = wk.mass + (int64_t)row * wk.n_cuts * kBins;
     send(part + blockIdx.x * kBins + tid, mass[tid]);
     VerCut& cut = wk.cuts[row];
-    if (!last_of(&cut.binned, wk.n_chunks, &sh)) return;
+    if (!last_of(&cut.binned, wk.n_cuts, &sh)) return;
     u64_t m = 0;
-#pragma unroll 8
-    for (int i = 0; i < wk.n_chunks; ++i) m += receive(part + i * kBins + tid);
+    constexpr int kRound = 8;
+    for (int i = 0; i < wk.n_cuts; i += kRound) {
+        u64_t x[kRound];
+#pragma unroll
+        for (int j = 0; j < kRound; ++j) x[j] = receive(part + min(i + j, wk.n_cuts - 1) * kBins + tid);
+#pragma unroll
+        for (int j = 0; j < kRound; ++j) m += i + j < wk.n_cuts ? x[j] : 0;
+    }
     const u64_t all = block_fold(m, red, [](u64_t x, u64_t y) { return x + y; });
     const double want = (double)fmaxf(a.top_p, 0.0f) * (double)all;
     u64_t target = (u64_t)want;
@@ -388,14 +396,15 @@ __global__ __launch_bounds__(kBlock) void k_ver_bins(const VerifyArgs a, const V
 // workgroup's threads), `before` is the mass above them. Narrows their keys by bins until few are left, which
 // are ranked, or one logit many times over, of which the k-th in index order is the last.
 struct Settle {
-    u64_t mass[kBins], red[kWavesPerBlock];
+    u64_t mass[kBins], red[(kCutThreads / kWave)];
     uint2 few[kFew];
     u64_t before;
+    uint2 end;  // of the last token kept
     uint32_t n, k_lo, k_hi;
     int bin;
 };
 template <class Each>
-__device__ void settle(Each each_of, u64_t before, u64_t target, float mx, float c, Settle& s, uint32_t& thr, int32_t& cut) {
+__device__ void settle(Each each_of, u64_t before, u64_t target, float mx, float c, Settle& s, float& thr, int32_t& cut) {
     const int tid = threadIdx.x;
     uint32_t lo = 0, hi = 0xFFFFFFFFu;
     auto inside = [&](float l) {
@@ -410,6 +419,7 @@ __device__ void settle(Each each_of, u64_t before, u64_t target, float mx, float
             s.k_hi = 0;
             s.bin = 0;
             s.before = before;
+            s.end = make_uint2(__float_as_uint(INFINITY), 0xFFFFFFFFu);  // none
         }
         s.mass[tid] = 0;
         __syncthreads();
@@ -421,8 +431,10 @@ __device__ void settle(Each each_of, u64_t before, u64_t target, float mx, float
             a = min(a, k);
             b = max(b, k);
         });
-        atomicMin(&s.k_lo, a);
-        atomicMax(&s.k_hi, b);
+        if (a <= b) {
+            atomicMin(&s.k_lo, a);
+            atomicMax(&s.k_hi, b);
+        }
         __syncthreads();
         if (s.n <= kFew || s.k_lo == s.k_hi) break;
         lo = s.k_lo;
@@ -455,7 +467,7 @@ __device__ void settle(Each each_of, u64_t before, u64_t target, float mx, float
             else
                 a = mid + 1;
         }
-        thr = key;
+        thr = l1;
         cut = a;
         return;
     }
@@ -469,25 +481,22 @@ __device__ void settle(Each each_of, u64_t before, u64_t target, float mx, float
             const uint32_t kj = logit_key(lj);
             if (kj > k || (kj == k && s.few[j].y < x)) sum += weight_fix(lj, mx, c);
         }
-        if (sum < target && sum + weight_fix(l, mx, c) >= target) {
-            s.k_lo = k;
-            s.k_hi = x;
-        }
+        if (sum < target && sum + weight_fix(l, mx, c) >= target) s.end = s.few[tid];
     }
     __syncthreads();
-    thr = s.k_lo;
-    cut = (int32_t)s.k_hi;
+    thr = __uint_as_float(s.end.x);
+    cut = (int32_t)s.end.y;
 }
 
-__global__ __launch_bounds__(kBlock) void k_ver_cut(const VerifyArgs a, const VerWork wk) {
+__global__ __launch_bounds__(kCutThreads) void k_ver_cut(const VerifyArgs a, const VerWork wk) {
     __shared__ uint2 list[kList];
     __shared__ Settle s;
     __shared__ uint32_t n_here, at_here;
     __shared__ int sh;
-    const int tid = threadIdx.x, row = blockIdx.y, x0 = blockIdx.x * kChunk, n = min(kChunk, a.vocab - x0);
+    const int tid = threadIdx.x, row = blockIdx.y, x0 = blockIdx.x * kCutChunk, n = min(kCutChunk, a.vocab - x0);
     const float* p = a.logits + (int64_t)row * a.ld;
-    float v[kChunkEach];
-    take<kChunkEach, false>(p + x0, n, NAN, v);
+    float v[kCutEach];
+    take<kCutEach, false>(p + x0, n, NAN, v);
     VerCut& cut = wk.cuts[row];
     const float mx = cut.mx;
     const int b0 = cut.bin;
@@ -498,28 +507,29 @@ __global__ __launch_bounds__(kBlock) void k_ver_cut(const VerifyArgs a, const Ve
     __syncthreads();
     double above = 0.0;
 #pragma unroll
-    for (int k = 0; k < kChunkEach; ++k) {
+    for (int k = 0; k < kCutEach; ++k) {
         const int b = v[k] <= mx ? bin(v[k]) : kBins;
-        if (b == b0) list[atomicAdd(&n_here, 1u)] = make_uint2(__float_as_uint(v[k]), (uint32_t)(x0 + place<kChunkEach, false>(k)));
+        if (b == b0) {
+            const uint32_t at = atomicAdd(&n_here, 1u);
+            if (at < kList) list[at] = make_uint2(__float_as_uint(v[k]), (uint32_t)(x0 + place<kCutEach, false>(k)));
+        }
         if (b < b0) above += weight(v[k], mx, c64);
     }
     above = block_sum(above, s.red);
     if (tid == 0) {
-        send(wk.above + (int64_t)row * wk.n_chunks + blockIdx.x, (u64_t)__double_as_longlong(above));
+        send(wk.above + (int64_t)row * wk.n_cuts + blockIdx.x, (u64_t)__double_as_longlong(above));
         at_here = n_here ? __hip_atomic_fetch_add(&cut.listed, n_here, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
     }
     __syncthreads();
-    for (uint32_t i = tid; i < n_here; i += kBlock)
+    for (uint32_t i = tid; i < min(n_here, (uint32_t)kList); i += kCutThreads)
         if (at_here + i < kList) send(wk.list + (int64_t)row * kList + at_here + i, (u64_t)list[i].y << 32 | list[i].x);
-    if (!last_of(&cut.done, wk.n_chunks, &sh)) return;
+    if (!last_of(&cut.done, wk.n_cuts, &sh)) return;
     const uint32_t m = __hip_atomic_load(&cut.listed, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     VerRow r;
     r.mx = mx;
     r.arg = 0;
-    r.thr = 0;
-    r.cut = INT_MAX;
     double z = 0.0;
-    for (int i = tid; i < wk.n_chunks; i += kBlock) z += __longlong_as_double((long long)receive(wk.above + (int64_t)row * wk.n_chunks + i));
+    for (int i = tid; i < wk.n_cuts; i += kCutThreads) z += __longlong_as_double((long long)receive(wk.above + (int64_t)row * wk.n_cuts + i));
     z = block_sum(z, s.red);
     double in = 0.0;
     auto settle_of = [&](auto each_of) {
@@ -529,13 +539,13 @@ __global__ __launch_bounds__(kBlock) void k_ver_cut(const VerifyArgs a, const Ve
         });
     };
     if (m <= kList) {
-        for (uint32_t i = tid; i < m; i += kBlock) {
+        for (uint32_t i = tid; i < m; i += kCutThreads) {
             const u64_t e = receive(wk.list + (int64_t)row * kList + i);
             list[i] = make_uint2((uint32_t)e, (uint32_t)(e >> 32));
         }
         __syncthreads();
         settle_of([&](auto f) {
-            for (uint32_t i = tid; i < m; i += kBlock) f((int)list[i].y, __uint_as_float(list[i].x));
+            for (uint32_t i = tid; i < m; i += kCutThreads) f((int)list[i].y, __uint_as_float(list[i].x));
         });
     } else {
         // too many for the list (one logit thousands of times over, or a bin that most logits are in): from the row
@@ -587,8 +597,8 @@ struct Left {
     double t, c;
     const int* gone;   // the rejected tokens (LDS), where there is no Q
     int n_gone;
-    __device__ double operator()(float lx, float qx, int x) const {
-        if (!kept(r, lx, x)) return 0.0;
+    // of token x, where it is kept
+    __device__ double of_kept(float lx, float qx, int x) const {
         const double w = weight(lx, r.mx, c);
         if (q) return fmax(w * r.inv_z - t * (double)qx, 0.0);
         for (int i = 0; i < n_gone; ++i)
@@ -597,23 +607,41 @@ struct Left {
     }
 };
 
-// The sum of a chunk of it, over the workgroup.
-template <int E>
-__device__ __forceinline__ double left_sum(const Left& f, int vocab, int chunk, u64_t* red) {
-    const int x0 = chunk * kChunk, n = min(kChunk, vocab - x0);
-    float l[E], q[E];
-    take<E, false>(f.l + x0, n, NAN, l);
-    if (f.q) take<E, false>(f.q + x0, n, 0.0f, q);
+// The sum of N chunks of it (those that there are), over the workgroup's threads; every chunk's loads go first.
+template <int E, int N>
+__device__ __forceinline__ double left_part(const Left& f, int vocab, int chunk) {
+    float l[N][E], q[N][E];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int x0 = (chunk + i) * kChunk, n = min(kChunk, vocab - x0);
+        take<E, false>(f.l + x0, n, NAN, l[i]);
+        if (f.q) take<E, false>(f.q + x0, n, 0.0f, q[i]);
+    }
     double sum = 0.0;
 #pragma unroll
-    for (int k = 0; k < E; ++k) sum += f(l[k], f.q ? q[k] : 0.0f, x0 + place<E, false>(k));
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+            const int x = (chunk + i) * kChunk + place<E, false>(k);
+            if (kept(f.r, l[i][k], x)) sum += f.of_kept(l[i][k], f.q ? q[i][k] : 0.0f, x);
+        }
+    return sum;
+}
+template <int E>
+__device__ __forceinline__ double left_sum(const Left& f, int vocab, int chunk, u64_t* red) {
+    return block_sum(left_part<E, 1>(f, vocab, chunk), red);
+}
+template <int E>
+__device__ double left_row_sum(const Left& f, int vocab, int n_chunks, u64_t* red) {
+    double sum = 0.0;
+    for (int ch = 0; ch < n_chunks; ch += 8) sum += left_part<E, 8>(f, vocab, ch);
     return block_sum(sum, red);
 }
 
 // The first token at which the running sum exceeds u times the total, from the chunks' sums (LDS). -1 where
-// nothing is left. Inside its chunk the sums run over the threads' consecutive tokens.
+// nothing is left. *p_out (LDS): P of it. Inside its chunk the sums run over the threads' consecutive tokens.
 template <int E>
-__device__ int draw(const Left& f, int vocab, const double* sums, int n_chunks, double u, u64_t* red, int* sh) {
+__device__ int draw(const Left& f, int vocab, const double* sums, int n_chunks, double u, u64_t* red, int* sh, double* p_out) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     __syncthreads();
     // every wave scans the chunks' sums: lane i holds those of 2 i and 2 i + 1
@@ -647,7 +675,7 @@ __device__ int draw(const Left& f, int vocab, const double* sums, int n_chunks, 
     if (f.q) take<E, true>(f.q + x0, n, 0.0f, q);
 #pragma unroll
     for (int k = 0; k < E; ++k) {
-        w[k] = f(l[k], f.q ? q[k] : 0.0f, x0 + at + k);
+        w[k] = kept(f.r, l[k], x0 + at + k) ? f.of_kept(l[k], f.q ? q[k] : 0.0f, x0 + at + k) : 0.0;
         mine += w[k];
     }
     double up = mine;
@@ -683,13 +711,18 @@ __device__ int draw(const Left& f, int vocab, const double* sums, int n_chunks, 
         atomicMax(&sh[1], last);
     }
     __syncthreads();
-    return x0 + (sh[0] == INT_MAX ? sh[1] : sh[0]);  // past the sums' rounding: the last token that is left
+    const int tok = sh[0] == INT_MAX ? sh[1] : sh[0];  // past the sums' rounding: the last token that is left
+#pragma unroll
+    for (int k = 0; k < E; ++k)
+        if (at + k == tok) *p_out = weight(l[k], f.r.mx, f.c) * f.r.inv_z;
+    __syncthreads();
+    return x0 + tok;
 }
 
-__device__ __forceinline__ void put_next(const VerifyArgs& a, const VerRow& r, const float* l, int tok, double c) {
+__device__ __forceinline__ void put_next(const VerifyArgs& a, int tok, double p) {
     if (threadIdx.x) return;
     a.result[1] = tok;
-    if (a.probs) a.probs[0] = (float)(a.temperature <= 0.0f ? 1.0 : prob(r, l[tok], tok, c));
+    if (a.probs) a.probs[0] = (float)p;
 }
 
 // ---------------------------------------------------------------- the walk
@@ -698,9 +731,11 @@ __global__ __launch_bounds__(kVerThreads) void k_ver_walk(const VerifyArgs a, co
     __shared__ VerRow rows[kTreeMax];
     __shared__ __align__(16) int parent[kTreeMax];
     __shared__ int token[kTreeMax], first[kTreeMax], gone[kTreeMax];
+    __shared__ float gone_l[kTreeMax];
     __shared__ double pc[kTreeMax], qc[kTreeMax], draws[kTreeMax], s1[kTreeMax], sums[kMaxChunks];
     __shared__ u64_t red[kVerWaves];
     __shared__ int sh[4];
+    __shared__ double p_next;
     const int tid = threadIdx.x, n = a.n_tree, V = a.vocab;
     const bool greedy = a.temperature <= 0.0f, cut = !greedy && a.top_p < 1.0f, sampled = a.draft && !greedy;
     const bool leader = blockIdx.x == 0;  // writes what all workgroups find alike
@@ -791,8 +826,7 @@ __global__ __launch_bounds__(kVerThreads) void k_ver_walk(const VerifyArgs a, co
                 double S = kids ? s1[at] : 1.0;
                 if (kids >= 2) {
                     const Left f = {rows[at], a.logits + (int64_t)at * a.ld, a.draft + (int64_t)at * a.ld_draft, t, c, nullptr, 0};
-                    S = 0.0;
-                    for (int ch = 0; ch < wk.n_chunks; ++ch) S += left_sum<kWalkEach>(f, V, ch, red);
+                    S = left_row_sum<kWalkEach>(f, V, wk.n_chunks, red);
                     const double left = pc[j] - t * qc[j];
                     if (left > 0.0 && draws[j] * qc[j] * S < left) {
                         next = j;
@@ -815,12 +849,13 @@ __global__ __launch_bounds__(kVerThreads) void k_ver_walk(const VerifyArgs a, co
         if (tid == 0) a.result[0] = count;
     }
     if (greedy) {
-        put_next(a, r, l, r.arg, c);
+        put_next(a, r.arg, 1.0);
         return;
     }
     // the next token, from what is left of row `at`
     if (!sampled && up == at) {
         gone[k] = token[tid];
+        gone_l[k] = lt;
         atomicMax(&sh[2], k + 1);
     }
     __syncthreads();
@@ -848,14 +883,14 @@ __global__ __launch_bounds__(kVerThreads) void k_ver_walk(const VerifyArgs a, co
             if (again) continue;
             const int ch = x / kChunk;
             const double old = sums[ch];
-            double now = old - weight(l[x], r.mx, c);
+            double now = old - weight(gone_l[i], r.mx, c);
             if (!(now > old * 0x1p-16)) now = left_sum<kWalkEach>(f, V, ch, red);
             __syncthreads();
             if (tid == 0) sums[ch] = now;
             __syncthreads();
         }
     }
-    int tok = draw<kWalkEach>(f, V, sums, wk.n_chunks, draws[0], red, sh);
+    int tok = draw<kWalkEach>(f, V, sums, wk.n_chunks, draws[0], red, sh, &p_next);
     if (tok < 0) {  // nothing is left: from P itself
         f.q = nullptr;
         f.n_gone = 0;
@@ -868,9 +903,9 @@ __global__ __launch_bounds__(kVerThreads) void k_ver_walk(const VerifyArgs a, co
         } else {
             chunk_sums();
         }
-        tok = draw<kWalkEach>(f, V, sums, wk.n_chunks, draws[0], red, sh);
+        tok = draw<kWalkEach>(f, V, sums, wk.n_chunks, draws[0], red, sh, &p_next);
     }
-    put_next(a, r, l, tok < 0 ? r.arg : tok, c);
+    put_next(a, tok < 0 ? r.arg : tok, tok < 0 ? 0.0 : p_next);
 }
 
 VerWork work_of(int n_tree, int vocab, void* ws, size_t* bytes) {
@@ -888,8 +923,9 @@ VerWork work_of(int n_tree, int vocab, void* ws, size_t* bytes) {
     w.cuts = (VerCut*)part(n * sizeof(VerCut));
     w.chunks = (VerChunk*)part(all * sizeof(VerChunk));
     w.round = (double*)part(all * sizeof(double));
-    w.mass = (u64_t*)part(all * kBins * sizeof(u64_t));
-    w.above = (u64_t*)part(all * sizeof(u64_t));
+    w.n_cuts = (vocab + kCutChunk - 1) / kCutChunk;
+    w.mass = (u64_t*)part(n * w.n_cuts * kBins * sizeof(u64_t));
+    w.above = (u64_t*)part(n * w.n_cuts * sizeof(u64_t));
     w.list = (u64_t*)part(n * kList * sizeof(u64_t));
     w.left = (u64_t*)part((size_t)w.n_chunks * sizeof(u64_t));
     if (bytes) *bytes = (size_t)(p - (char*)ws);
@@ -913,8 +949,9 @@ hipError_t launch_verify(const VerifyArgs& a, void* ws, hipStream_t st) {
         return hipGetLastError();
     };
     hipError_t e = launch(k_ver_chunks, grid, kBlock);
-    if (e == hipSuccess && cut) e = launch(k_ver_bins, grid, kBlock);
-    if (e == hipSuccess && cut) e = launch(k_ver_cut, grid, kBlock);
+    const dim3 cuts((unsigned)wk.n_cuts, (unsigned)a.n_tree);
+    if (e == hipSuccess && cut) e = launch(k_ver_bins, cuts, kCutThreads);
+    if (e == hipSuccess && cut) e = launch(k_ver_cut, cuts, kCutThreads);
     if (e == hipSuccess && sampled) e = launch(k_ver_rounds, grid, kBlock);
     if (e == hipSuccess) e = launch(k_ver_walk, dim3(cut || sampled ? (unsigned)wk.n_chunks : 1u), kVerThreads);
     return e;
