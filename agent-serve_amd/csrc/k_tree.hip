@@ -22,6 +22,7 @@
 // threads load, scale and store keys, half values, one step ahead of the products; loads are two
 // steps ahead. Splits are merged by k_tree_merge; one split writes the output itself.
 #include <algorithm>
+#include <type_traits>
 
 #include "dev_common.hpp"
 #include "tf_internal.hpp"
@@ -49,17 +50,42 @@ __device__ __forceinline__ int v_entry(int dim, int dt, int kg) {
     return 16 * kg + 8 * b3 + ((dim & 7) ^ b3 ^ (dt << 1 & 6));
 }
 
+// Eight numbers x(j), times sc in the second form, as fp16 pairs. The rest of a number is one mixed-precision
+// fma (number x 1 - its half); written out, the compiler widens the half first.
+template <class X>
+__device__ __forceinline__ void split8(X x, h8_t& hi, h8_t& lo) {
+    typedef float f2_t __attribute__((ext_vector_type(2)));
+    typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const f2_t y = {x(2 * j), x(2 * j + 1)};
+        h[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(y, h2_t));
+        f2_t r;
+        asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel_hi:[0,0,1]" : "=v"(r.x) : "v"(y.x), "v"(h[j]));
+        asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "=v"(r.y) : "v"(y.y), "v"(h[j]));
+        l[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, h2_t));
+    }
+    __builtin_memcpy(&hi, h, 16);
+    __builtin_memcpy(&lo, l, 16);
+}
+template <class X>
+__device__ __forceinline__ void split8(X x, float sc, h8_t& hi, h8_t& lo) {
+    split8([&](int j) { return x(j) * sc; }, hi, lo);
+}
+
 template <class T, int HP, int WR, int WP, int QS, bool EXACT>
 __global__ __launch_bounds__(64 * WR * WP) void k_tree_attn(const TreeAttnArgs a) {
     constexpr bool kPair = sizeof(T) == 4;
-    constexpr int NW = WR * WP, NC = HP / 32, NT = HP / 16;
-    constexpr int F = HP / WR;       // elements a thread loads per step
-    constexpr int DV = F / 8;        // dims of 8 values each
+    constexpr int NW = WR * WP, NC = HP / 32, NT = HP / 16, kE = (int)sizeof(T);
+    constexpr int kUnits = HP / WR / 8;  // units of 8 key elements a thread loads per step
+    // dims of 8 values each a thread loads per step: at least a word of them (then some threads load none)
+    constexpr int DV = HP / WR / 8 > 4 / kE ? HP / WR / 8 : 4 / kE;
+    constexpr int kWords = (kUnits > DV ? kUnits : DV) * 8 * kE / 4;
     constexpr int kFrag = kPair ? 2048 : 1024;  // bytes of a fragment: hi, then lo
     constexpr int kKeys = 2 * NC * kFrag, REC = kKeys + NT * kFrag;
-    constexpr int BN = kRec * WP;
-    constexpr int kBufs = 2;
-    static_assert(NW % 2 == 0 && F % 8 == 0, "half of the waves load keys, half values");
+    constexpr int BN = kRec * WP, kBufs = 2;
+    static_assert(NW % 2 == 0 && HP / WR >= 8, "half of the waves load keys, half values");
     constexpr int kMergeWords = QS * (4 * NT + 2);
     constexpr int kRecords = kBufs * WP * REC, kMerge = WR * (WP - 1) * 64 * kMergeWords * 4;
     __shared__ __align__(16) unsigned char lds[kRecords > kMerge ? kRecords : kMerge];
@@ -75,74 +101,89 @@ __global__ __launch_bounds__(64 * WR * WP) void k_tree_attn(const TreeAttnArgs a
     const int end = a.n_past + a.n_tree;
     const int units = (end + BN - 1) / BN, per = (units + a.S - 1) / a.S;
     const int u0 = split * per, steps = min(units - u0, per);
-    const int64_t stride = a.layout == TF_HIP_KV_HEAD_MAJOR ? hd : (int64_t)a.G * hd;  // elements a position
+    const int stride = a.layout == TF_HIP_KV_HEAD_MAJOR ? hd : a.G * hd;  // elements a position
     const int64_t base = kv_offset(a.layout, a.G, a.max_seq, hd, g, 0);
 
     // ---- loads
     // Keys: a wave's unit is 16 positions x 32 dims of a fragment, lane = (position lane / 4, 8 dims from
     // 8 (lane % 4)), which is entry 16 (lane % 4) + (position ^ 2 (lane % 4)). Values: a thread holds the
     // 8 positions of a key group (4 kg + 0..3 and 16 + 4 kg + 0..3, as the weights lie in the lanes) of
-    // DV dims.
+    // DV dims. A step's base is uniform and a thread's places in it are 32-bit offsets, found again for a
+    // step past the end, which repeats the last row.
     constexpr int kHalf = NW / 2;
     const bool key_wave = wave < kHalf;
     const int tv = tid - 64 * kHalf;  // value threads
     const int v_d = DV * (tv % (HP / DV)), v_kg = tv / (HP / DV) % 4, v_rec = tv / (4 * (HP / DV));
-    const T* src = (const T*)(key_wave ? a.kc : a.vc) + base;
-    T reg[F];
-    auto load8 = [&](const T* p, bool ok, T* to) {  // 8 elements at a multiple of 8
-        if constexpr (kPair) {
-            const float4 x = ok ? gload_f4(p) : make_float4(0, 0, 0, 0), y = ok ? gload_f4(p + 4) : make_float4(0, 0, 0, 0);
-            to[0] = x.x; to[1] = x.y; to[2] = x.z; to[3] = x.w;
-            to[4] = y.x; to[5] = y.y; to[6] = y.z; to[7] = y.w;
-        } else {
-            const uint4 x = ok ? gload_u4(p) : make_uint4(0, 0, 0, 0);
-            __builtin_memcpy(to, &x, 16);
-        }
+    const char* src = (const char*)((const T*)(key_wave ? a.kc : a.vc) + base);
+    uint32_t raw[kWords];
+    auto element = [&](int i) __attribute__((always_inline)) -> float {
+        if constexpr (kPair)
+            return __uint_as_float(raw[i]);
+        else
+            return h2f(i & 1 ? raw[i / 2] >> 16 : raw[i / 2] & 0xFFFFu);
     };
-    auto load = [&](int step) {
-        const int p = BN * (u0 + step);
+    auto key_dim = [&](int u) { return 32 * ((wave * kUnits + u) % NC) + 8 * (lane & 3); };
+    uint32_t off[kUnits > 8 ? kUnits : 8];
+    auto places = [&](int most) __attribute__((always_inline)) {  // most: the step's last position
         if (key_wave) {
 #pragma unroll
-            for (int u = 0; u < F / 8; ++u) {
-                const int wu = wave * (F / 8) + u;  // (record, half, chunk)
-                const int c = wu % NC, pos = p + 16 * (wu / NC) + (lane >> 2), d = 32 * c + 8 * (lane & 3);
-                load8(src + (int64_t)min(pos, end - 1) * stride + d, EXACT || d < hd, reg + 8 * u);
+            for (int u = 0; u < kUnits; ++u) {
+                const int pos = min(16 * ((wave * kUnits + u) / NC) + (lane >> 2), most), d = key_dim(u);
+                off[u] = (uint32_t)(pos * stride + (EXACT || d < hd ? d : 0)) * kE;
             }
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int pos = min(p + kRec * v_rec + 4 * v_kg + (j < 4 ? j : 12 + j), end - 1);
-                const T* q = src + (int64_t)pos * stride + v_d;
-                T* to = reg + j * DV;
-                const bool ok = EXACT || v_d < hd;
-                if constexpr (DV == 8) {
-                    load8(q, ok, to);
-                } else if constexpr (DV * sizeof(T) == 16) {
-                    const uint4 x = ok ? gload_u4(q) : make_uint4(0, 0, 0, 0);
-                    __builtin_memcpy(to, &x, 16);
-                } else if constexpr (DV * sizeof(T) == 8) {
-                    const uint2 x = ok ? gload_u2(q) : make_uint2(0, 0);
-                    __builtin_memcpy(to, &x, 8);
-                } else if constexpr (DV * sizeof(T) == 4) {
-                    const uint32_t x = ok ? *(const TF_GLOBAL uint32_t*)q : 0u;
-                    __builtin_memcpy(to, &x, 4);
-                } else {
-                    to[0] = ok ? *gptr(q) : (T)0;
-                }
+                const int pos = min(kRec * v_rec + 4 * v_kg + (j < 4 ? j : 12 + j), most);
+                off[j] = (uint32_t)(pos * stride + (EXACT || v_d < hd ? v_d : 0)) * kE;
             }
         }
     };
+    auto words = [&](const char* q, uint32_t* to, auto n) __attribute__((always_inline)) {
+        if constexpr (n() >= 4) {
+#pragma unroll
+            for (int i = 0; i < n(); i += 4) {
+                const uint4 x = gload_u4(q + 4 * i);
+                to[i] = x.x; to[i + 1] = x.y; to[i + 2] = x.z; to[i + 3] = x.w;
+            }
+        } else if constexpr (n() == 2) {
+            const uint2 x = gload_u2(q);
+            to[0] = x.x; to[1] = x.y;
+        } else {
+            to[0] = *(const TF_GLOBAL uint32_t*)q;
+        }
+    };
+    auto load = [&](int step) __attribute__((always_inline)) {
+        const int p = BN * (u0 + step);
+        if (p + BN > end) places(end - 1 - p);
+        const char* at = src + (int64_t)p * stride * kE;
+        if (key_wave) {
+#pragma unroll
+            for (int u = 0; u < kUnits; ++u) {
+                words(at + off[u], raw + u * 2 * kE, std::integral_constant<int, 2 * kE>());
+                if (!EXACT && key_dim(u) >= hd)
+#pragma unroll
+                    for (int i = 0; i < 2 * kE; ++i) raw[u * 2 * kE + i] = 0;
+            }
+        } else if (v_rec < WP) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) words(at + off[j], raw + j * DV * kE / 4, std::integral_constant<int, DV * kE / 4>());
+            if (!EXACT && v_d >= hd)
+#pragma unroll
+                for (int i = 0; i < 2 * DV * kE; ++i) raw[i] = 0;
+        }
+    };
     // the largest finite magnitude of this wave's elements, for their scale
-    auto publish = [&](int step) {
+    auto publish = [&](int step) __attribute__((always_inline)) {
         if constexpr (kPair) {
             float m = 0.0f;
 #pragma unroll
-            for (int i = 0; i < F; ++i) m = fmaxf(m, fabsf((float)reg[i]));
+            for (int i = 0; i < kWords; ++i) m = fmaxf(m, fabsf(__uint_as_float(raw[i])));
             if (!(m < INFINITY)) {
                 m = 0.0f;
 #pragma unroll
-                for (int i = 0; i < F; ++i) {
-                    const float x = fabsf((float)reg[i]);
+                for (int i = 0; i < kWords; ++i) {
+                    const float x = fabsf(__uint_as_float(raw[i]));
                     if (x < INFINITY) m = fmaxf(m, x);
                 }
             }
@@ -167,72 +208,69 @@ __global__ __launch_bounds__(64 * WR * WP) void k_tree_attn(const TreeAttnArgs a
             ev_min = min(ev_min, ev);
         }
     };
-    auto put8 = [&](unsigned char* to, const T* x, float sc) {
-        h8_t hi;
-        if constexpr (kPair) {
-            h8_t lo;
+    // Infinities and NaN among `n` elements from i are taken out; whether there were any.
+    auto clean = [&](int i, int n) __attribute__((always_inline)) {
+        bool odd = false;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float y = (float)x[j] * sc;
-                hi[j] = (_Float16)y;
-                lo[j] = (_Float16)(y - (float)hi[j]);
-            }
-            *(h8_t*)(to + 1024) = lo;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) hi[j] = x[j];
+        for (int k = i; k < i + n; ++k) {
+            if (fabsf(element(k)) < INFINITY) continue;
+            odd = true;
+            if constexpr (kPair)
+                raw[k] = 0;
+            else
+                raw[k / 2] &= k & 1 ? 0xFFFFu : 0xFFFF0000u;
         }
-        *(h8_t*)to = hi;
+        return odd;
     };
     // The loaded step as records. A step that reaches into the tree takes its infinities and NaN out and
     // notes their positions: a zero weight times one of them would be NaN in the rows that do not see it.
-    auto store = [&](int step) {
+    auto store = [&](int step) __attribute__((always_inline)) {
         unsigned char* buf = lds + (step & 1) * WP * REC;
         const bool tree = BN * (u0 + step + 1) > a.n_past;
-        const float sc = kPair ? pow2f(key_wave ? ek : ev) : 1.0f;
         if (key_wave) {
 #pragma unroll
-            for (int u = 0; u < F / 8; ++u) {
-                const int wu = wave * (F / 8) + u, rec = wu / (2 * NC), hc = wu % (2 * NC);
-                if (tree) {
-                    bool fine = true;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const bool ok = fabsf((float)reg[8 * u + j]) < INFINITY;
-                        fine = fine && ok;
-                        reg[8 * u + j] = ok ? reg[8 * u + j] : (T)0;
-                    }
-                    if (!fine) atomicOr(&bad[step % 3][rec], 1u << (16 * (hc / NC) + (lane >> 2)));
-                }
-                const int ch = lane & 3;
-                put8(buf + rec * REC + hc * kFrag + 16 * (16 * ch + ((lane >> 2) ^ (2 * ch))), reg + 8 * u, sc);
-            }
-        } else {
-            if (tree) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    bool fine = true;
-#pragma unroll
-                    for (int i = 0; i < DV; ++i) {
-                        const bool ok = fabsf((float)reg[j * DV + i]) < INFINITY;
-                        fine = fine && ok;
-                        reg[j * DV + i] = ok ? reg[j * DV + i] : (T)0;
-                    }
-                    if (!fine) atomicOr(&bad[step % 3][v_rec], 1u << (4 * v_kg + (j < 4 ? j : 12 + j)));
+            for (int u = 0; u < kUnits; ++u) {
+                const int wu = wave * kUnits + u, rec = wu / (2 * NC), hc = wu % (2 * NC), ch = lane & 3;
+                if (tree && clean(8 * u, 8)) atomicOr(&bad[step % 3][rec], 1u << (16 * (hc / NC) + (lane >> 2)));
+                unsigned char* to = buf + rec * REC + hc * kFrag + 16 * (16 * ch + ((lane >> 2) ^ (2 * ch)));
+                if constexpr (kPair) {
+                    h8_t hi, lo;
+                    split8([&](int j) { return __uint_as_float(raw[8 * u + j]); }, pow2f(ek), hi, lo);
+                    *(h8_t*)to = hi;
+                    *(h8_t*)(to + 1024) = lo;
+                } else {
+                    *(uint4*)to = make_uint4(raw[4 * u], raw[4 * u + 1], raw[4 * u + 2], raw[4 * u + 3]);
                 }
             }
+        } else if (v_rec < WP) {
+            if (tree)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (clean(j * DV, DV)) atomicOr(&bad[step % 3][v_rec], 1u << (4 * v_kg + (j < 4 ? j : 12 + j)));
 #pragma unroll
             for (int i = 0; i < DV; ++i) {
-                T x[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = reg[j * DV + i];
                 const int d = v_d + i, dt = d >> 4;
-                put8(buf + v_rec * REC + kKeys + dt * kFrag + 16 * v_entry(d & 15, dt, v_kg), x, sc);
+                unsigned char* to = buf + v_rec * REC + kKeys + dt * kFrag + 16 * v_entry(d & 15, dt, v_kg);
+                if constexpr (kPair) {
+                    h8_t hi, lo;
+                    split8([&](int j) { return __uint_as_float(raw[j * DV + i]); }, pow2f(ev), hi, lo);
+                    *(h8_t*)to = hi;
+                    *(h8_t*)(to + 1024) = lo;
+                } else {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)  // halves i of positions 2 j and 2 j + 1
+                        w[j] = __builtin_amdgcn_perm(raw[((2 * j + 1) * DV + i) / 2], raw[(2 * j * DV + i) / 2], i & 1 ? 0x07060302u : 0x05040100u);
+                    *(uint4*)to = make_uint4(w[0], w[1], w[2], w[3]);
+                }
             }
         }
     };
 
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) raw[i] = 0;
     if (tid < 3 * WP) bad[tid / WP][tid % WP] = 0;
+    places(BN - 1);
     load(0);
 
     // ---- the wave's queries: lane l holds row l % 16 of each subtile, dims 32 c + 8 (l / 16) ..
@@ -263,22 +301,14 @@ __global__ __launch_bounds__(64 * WR * WP) void k_tree_attn(const TreeAttnArgs a
 #pragma unroll
             for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[c][j]));
         }
-        m = quad_max(m);
-        const int e = scale_exp(m);
-        const float sc = pow2f(e);
+        const int e = scale_exp(quad_max(m));
         fq[qs] = ldexpf(kLog2e / sqrtf((float)hd), -e);  // scores in units of log2
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float x = v[c][j] * sc;
-                qh[qs][c][j] = (_Float16)x;
-                ql[qs][c][j] = (_Float16)(x - (float)qh[qs][c][j]);
-            }
+        for (int c = 0; c < NC; ++c) split8([&](int j) { return v[c][j]; }, pow2f(e), qh[qs][c], ql[qs][c]);
     }
     f4_t acc[QS][NT];  // O 2^(unit + 14)
     float m_run[QS], l_run[QS];  // l of this lane's positions
-    int unit = 126;
+    int unit = kPair ? 126 : 0;
 #pragma unroll
     for (int qs = 0; qs < QS; ++qs) {
         m_run[qs] = -INFINITY;
@@ -291,8 +321,8 @@ __global__ __launch_bounds__(64 * WR * WP) void k_tree_attn(const TreeAttnArgs a
 #pragma unroll
     for (int i = 0; i < 4; ++i) v_at[i] = 16 * v_entry(l16, i, gq);
 
-    // ---- one record: ke and ve its scales
-    auto record = [&](int step, int ke, int ve) {
+    // ---- one record: ke and ve its scales; TREE: it reaches into the tree
+    auto record = [&](auto TREE, int step, int ke, int ve) __attribute__((always_inline)) {
         const unsigned char* rec = lds + ((step & 1) * WP + wp) * REC;
         const int p = BN * (u0 + step) + kRec * wp;
         f4_t s[QS][2];
@@ -305,28 +335,32 @@ __global__ __launch_bounds__(64 * WR * WP) void k_tree_attn(const TreeAttnArgs a
                 const unsigned char* f = rec + (half * NC + c) * kFrag + k_at;
                 const h8_t kh = *(const h8_t*)f;
 #pragma unroll
-                for (int qs = 0; qs < QS; ++qs) {
-                    s[qs][half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[qs][c], s[qs][half], 0, 0, 0);
-                    s[qs][half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[qs][c], s[qs][half], 0, 0, 0);
-                }
+                for (int qs = 0; qs < QS; ++qs) s[qs][half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[qs][c], s[qs][half], 0, 0, 0);
+#pragma unroll
+                for (int qs = 0; qs < QS; ++qs) s[qs][half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[qs][c], s[qs][half], 0, 0, 0);
                 if constexpr (kPair) {
                     const h8_t kl = *(const h8_t*)(f + 1024);
 #pragma unroll
-                    for (int qs = 0; qs < QS; ++qs)
-                        s[qs][half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[qs][c], s[qs][half], 0, 0, 0);
+                    for (int qs = 0; qs < QS; ++qs) s[qs][half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[qs][c], s[qs][half], 0, 0, 0);
                 }
             }
-        const bool tree = p + kRec > a.n_past;
+        // the values are read ahead of the softmax, whose branches they would otherwise wait behind
+        h8_t vh[NT];
+#pragma unroll
+        for (int d = 0; d < NT; ++d) vh[d] = *(const h8_t*)(rec + kKeys + d * kFrag + v_at[d & 3]);
+#pragma unroll
+        for (int d = 0; d < NT; ++d) asm volatile("" : "+v"(vh[d]));
         uint32_t bits[QS], odd = 0;
-        if (tree) {
+        if constexpr (TREE()) {
             // bit b: the row sees position p + b
             odd = bad[step % 3][wp];
             const int off = p - a.n_past, left = end - p;
 #pragma unroll
             for (int qs = 0; qs < QS; ++qs) {
                 const uint64_t* m = a.masks + (int64_t)(min(row[qs], rows - 1) / rep) * a.mask_words;
-                uint64_t x;
-                if (off < 0) {
+                uint64_t x = ~0ull;
+                if (off <= -kRec) {
+                } else if (off < 0) {
                     x = (m[0] << -off) | ((1ull << -off) - 1);
                 } else {
                     const int w = off >> 6, sh = off & 63;
@@ -337,12 +371,10 @@ __global__ __launch_bounds__(64 * WR * WP) void k_tree_attn(const TreeAttnArgs a
             }
         }
         // values smaller than an earlier step's: the weights shrink; larger ones: the output does
-        int e = unit, shift = kWeightExp;
+        int e = 0, shift = kWeightExp;
         if constexpr (kPair) {
             e = min(unit, ve);
             shift = kWeightExp + e - ve;
-        } else {
-            e = 0;
         }
         const int de = e - unit;
         unit = e;
@@ -355,7 +387,7 @@ __global__ __launch_bounds__(64 * WR * WP) void k_tree_attn(const TreeAttnArgs a
             float x[8], mt = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] = s[qs][j >> 2][j & 3];
-            if (tree) {
+            if constexpr (TREE()) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int b = 4 * gq + (j < 4 ? j : 12 + j);
@@ -373,11 +405,10 @@ __global__ __launch_bounds__(64 * WR * WP) void k_tree_attn(const TreeAttnArgs a
             float ls = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float y = __builtin_amdgcn_exp2f(fmaf(x[j], f, sh));
-                ls += y;
-                ph[qs][j] = (_Float16)y;
-                pl[qs][j] = (_Float16)(y - (float)ph[qs][j]);
+                x[j] = __builtin_amdgcn_exp2f(fmaf(x[j], f, sh));
+                ls += x[j];
             }
+            split8([&](int j) { return x[j]; }, ph[qs], pl[qs]);
             l_run[qs] = fmaf(l_run[qs], alpha, kPair ? ldexpf(ls, -shift) : ls * pow2f(-kWeightExp));
             m_run[qs] = m_new;
             resc[qs] = kPair ? ldexpf(alpha, de) : alpha;
@@ -390,18 +421,14 @@ __global__ __launch_bounds__(64 * WR * WP) void k_tree_attn(const TreeAttnArgs a
                 for (int d = 0; d < NT; ++d) acc[qs][d] = acc[qs][d] * resc[qs];
 #pragma unroll
         for (int d = 0; d < NT; ++d) {
-            const unsigned char* f = rec + kKeys + d * kFrag + v_at[d & 3];
-            const h8_t vh = *(const h8_t*)f;
 #pragma unroll
-            for (int qs = 0; qs < QS; ++qs) {
-                acc[qs][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[qs], acc[qs][d], 0, 0, 0);
-                acc[qs][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl[qs], acc[qs][d], 0, 0, 0);
-            }
+            for (int qs = 0; qs < QS; ++qs) acc[qs][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh[d], ph[qs], acc[qs][d], 0, 0, 0);
+#pragma unroll
+            for (int qs = 0; qs < QS; ++qs) acc[qs][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh[d], pl[qs], acc[qs][d], 0, 0, 0);
             if constexpr (kPair) {
-                const h8_t vl = *(const h8_t*)(f + 1024);
+                const h8_t vl = *(const h8_t*)(rec + kKeys + d * kFrag + v_at[d & 3] + 1024);
 #pragma unroll
-                for (int qs = 0; qs < QS; ++qs)
-                    acc[qs][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[qs], acc[qs][d], 0, 0, 0);
+                for (int qs = 0; qs < QS; ++qs) acc[qs][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[qs], acc[qs][d], 0, 0, 0);
             }
         }
     };
@@ -417,19 +444,23 @@ __global__ __launch_bounds__(64 * WR * WP) void k_tree_attn(const TreeAttnArgs a
     }
     __syncthreads();
     // step t: records t are complete, and the loads of t + 1 with their scale
-    for (int t = 0; t < steps; ++t) {
+    auto step = [&](auto TREE, int t) __attribute__((always_inline)) {
         if (t + 1 < steps) {
             scales(t + 1);
             store(t + 1);
         }
         if (tid < WP) bad[(t + 2) % 3][tid] = 0;
         if (t + 2 < steps) load(t + 2);
-        if (BN * (u0 + t) + kRec * wp < end) record(t, ke, ve);
+        if (!TREE() || BN * (u0 + t) + kRec * wp < end) record(TREE, t, ke, ve);
         ke = ek;
         ve = ev;
         if (t + 2 < steps) publish(t + 2);
         if (t + 1 < steps) __syncthreads();
-    }
+    };
+    const int plain = max(0, min(steps, a.n_past / BN - u0));  // steps below n_past
+    int t = 0;
+    for (; t < plain; ++t) step(std::false_type(), t);
+    for (; t < steps; ++t) step(std::true_type(), t);
 
     // ---- the WP waves of a row group, then the row's 4 lanes
 #pragma unroll
@@ -471,7 +502,7 @@ __global__ __launch_bounds__(64 * WR * WP) void k_tree_attn(const TreeAttnArgs a
             }
             m_run[qs] = M;
         }
-    } else {
+    } else if constexpr (kPair) {
 #pragma unroll
         for (int qs = 0; qs < QS; ++qs)
 #pragma unroll
