@@ -16,11 +16,10 @@
 // The softmax's running reference is the score's maximum in units of log2, rounded up to a whole
 // number: rescaling by 2^(old - new) is exact, and it is needed only when the maximum passes one.
 //
-// A workgroup takes 16 QS WR rows of one kv head and one split of the positions, 32 WP positions
-// at a time, each 32 a record in LDS in fragment order: wave (wr, wp) runs rows of group wr over
-// record wp of every step, and the WP waves of a row group are merged at the end. Half of the
-// threads load, scale and store keys, half values, one step ahead of the products; loads are two
-// steps ahead. Splits are merged by k_tree_merge; one split writes the output itself.
+// A workgroup of NW waves takes 16 QS rows of one kv head a wave and one split of the positions, 32 at a
+// time (a step): the step's keys and values lie in LDS in fragment order (a record), and every wave runs its
+// rows over them. Half of the threads load, scale and store keys, half values, one step ahead of the
+// products; loads are two steps ahead. Splits are merged by k_tree_merge; one split writes the output itself.
 #include <algorithm>
 #include <type_traits>
 
@@ -74,32 +73,29 @@ __device__ __forceinline__ void split8(X x, float sc, h8_t& hi, h8_t& lo) {
     split8([&](int j) { return x(j) * sc; }, hi, lo);
 }
 
-template <class T, int HP, int WR, int WP, int QS, bool EXACT>
-__global__ __launch_bounds__(64 * WR * WP) void k_tree_attn(const TreeAttnArgs a) {
+template <class T, int HP, int NW, int QS, bool EXACT>
+__global__ __launch_bounds__(64 * NW) void k_tree_attn(const TreeAttnArgs a) {
     constexpr bool kPair = sizeof(T) == 4;
-    constexpr int NW = WR * WP, NC = HP / 32, NT = HP / 16, kE = (int)sizeof(T);
-    constexpr int kUnits = HP / WR / 8;  // units of 8 key elements a thread loads per step
+    constexpr int NC = HP / 32, NT = HP / 16, kE = (int)sizeof(T);
+    constexpr int kUnits = HP / NW / 8;  // units of 8 key elements a thread loads per step
     // dims of 8 values each a thread loads per step: at least a word of them (then some threads load none)
-    constexpr int DV = HP / WR / 8 > 4 / kE ? HP / WR / 8 : 4 / kE;
+    constexpr int DV = HP / NW / 8 > 4 / kE ? HP / NW / 8 : 4 / kE;
     constexpr int kWords = (kUnits > DV ? kUnits : DV) * 8 * kE / 4;
     constexpr int kFrag = kPair ? 2048 : 1024;  // bytes of a fragment: hi, then lo
     constexpr int kKeys = 2 * NC * kFrag, REC = kKeys + NT * kFrag;
-    constexpr int BN = kRec * WP, kBufs = 2;
-    static_assert(NW % 2 == 0 && HP / WR >= 8, "half of the waves load keys, half values");
-    constexpr int kMergeWords = QS * (4 * NT + 2);
-    constexpr int kRecords = kBufs * WP * REC, kMerge = WR * (WP - 1) * 64 * kMergeWords * 4;
-    __shared__ __align__(16) unsigned char lds[kRecords > kMerge ? kRecords : kMerge];
+    constexpr int kBufs = 2;
+    static_assert(NW % 2 == 0 && HP / NW >= 8, "half of the waves load keys, half values");
+    __shared__ __align__(16) unsigned char lds[kBufs * REC];
     __shared__ float amax[2][NW];
-    __shared__ uint32_t bad[3][WP];  // positions of a record with an infinity or NaN, by step mod 3
+    __shared__ uint32_t bad[3];  // positions of a record with an infinity or NaN, by step mod 3
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wr = wave % WR, wp = wave / WR;
     const int l16 = lane & 15, gq = lane >> 4;
     const int hd = EXACT ? HP : a.hd, rep = a.H / a.G, rows = a.n_tree * rep;
     // kv head fastest, then split, then row block: the row blocks of one span of keys are G S apart
     const int g = blockIdx.x % a.G, split = blockIdx.x / a.G % a.S, blk = blockIdx.x / (a.G * a.S);
     const int end = a.n_past + a.n_tree;
-    const int units = (end + BN - 1) / BN, per = (units + a.S - 1) / a.S;
+    const int units = (end + kRec - 1) / kRec, per = (units + a.S - 1) / a.S;
     const int u0 = split * per, steps = min(units - u0, per);
     const int stride = a.layout == TF_HIP_KV_HEAD_MAJOR ? hd : a.G * hd;  // elements a position
     const int64_t base = kv_offset(a.layout, a.G, a.max_seq, hd, g, 0);
@@ -113,7 +109,7 @@ __global__ __launch_bounds__(64 * WR * WP) void k_tree_attn(const TreeAttnArgs a
     constexpr int kHalf = NW / 2;
     const bool key_wave = wave < kHalf;
     const int tv = tid - 64 * kHalf;  // value threads
-    const int v_d = DV * (tv % (HP / DV)), v_kg = tv / (HP / DV) % 4, v_rec = tv / (4 * (HP / DV));
+    const int v_d = DV * (tv % (HP / DV)), v_kg = tv / (HP / DV);
     const char* src = (const char*)((const T*)(key_wave ? a.kc : a.vc) + base);
     uint32_t raw[kWords];
     auto element = [&](int i) __attribute__((always_inline)) -> float {
@@ -134,7 +130,7 @@ __global__ __launch_bounds__(64 * WR * WP) void k_tree_attn(const TreeAttnArgs a
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int pos = min(kRec * v_rec + 4 * v_kg + (j < 4 ? j : 12 + j), most);
+                const int pos = min(4 * v_kg + (j < 4 ? j : 12 + j), most);
                 off[j] = (uint32_t)(pos * stride + (EXACT || v_d < hd ? v_d : 0)) * kE;
             }
         }
@@ -154,8 +150,8 @@ __global__ __launch_bounds__(64 * WR * WP) void k_tree_attn(const TreeAttnArgs a
         }
     };
     auto load = [&](int step) __attribute__((always_inline)) {
-        const int p = BN * (u0 + step);
-        if (p + BN > end) places(end - 1 - p);
+        const int p = kRec * (u0 + step);
+        if (p + kRec > end) places(end - 1 - p);
         const char* at = src + (int64_t)p * stride * kE;
         if (key_wave) {
 #pragma unroll
@@ -165,7 +161,7 @@ __global__ __launch_bounds__(64 * WR * WP) void k_tree_attn(const TreeAttnArgs a
 #pragma unroll
                     for (int i = 0; i < 2 * kE; ++i) raw[u * 2 * kE + i] = 0;
             }
-        } else if (v_rec < WP) {
+        } else if (v_kg < 4) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) words(at + off[j], raw + j * DV * kE / 4, std::integral_constant<int, DV * kE / 4>());
             if (!EXACT && v_d >= hd)
@@ -225,14 +221,14 @@ __global__ __launch_bounds__(64 * WR * WP) void k_tree_attn(const TreeAttnArgs a
     // The loaded step as records. A step that reaches into the tree takes its infinities and NaN out and
     // notes their positions: a zero weight times one of them would be NaN in the rows that do not see it.
     auto store = [&](int step) __attribute__((always_inline)) {
-        unsigned char* buf = lds + (step & 1) * WP * REC;
-        const bool tree = BN * (u0 + step + 1) > a.n_past;
+        unsigned char* buf = lds + (step & 1) * REC;
+        const bool tree = kRec * (u0 + step + 1) > a.n_past;
         if (key_wave) {
 #pragma unroll
             for (int u = 0; u < kUnits; ++u) {
-                const int wu = wave * kUnits + u, rec = wu / (2 * NC), hc = wu % (2 * NC), ch = lane & 3;
-                if (tree && clean(8 * u, 8)) atomicOr(&bad[step % 3][rec], 1u << (16 * (hc / NC) + (lane >> 2)));
-                unsigned char* to = buf + rec * REC + hc * kFrag + 16 * (16 * ch + ((lane >> 2) ^ (2 * ch)));
+                const int hc = wave * kUnits + u, ch = lane & 3;  // (half, chunk)
+                if (tree && clean(8 * u, 8)) atomicOr(&bad[step % 3], 1u << (16 * (hc / NC) + (lane >> 2)));
+                unsigned char* to = buf + hc * kFrag + 16 * (16 * ch + ((lane >> 2) ^ (2 * ch)));
                 if constexpr (kPair) {
                     h8_t hi, lo;
                     split8([&](int j) { return __uint_as_float(raw[8 * u + j]); }, pow2f(ek), hi, lo);
@@ -242,15 +238,15 @@ __global__ __launch_bounds__(64 * WR * WP) void k_tree_attn(const TreeAttnArgs a
                     *(uint4*)to = make_uint4(raw[4 * u], raw[4 * u + 1], raw[4 * u + 2], raw[4 * u + 3]);
                 }
             }
-        } else if (v_rec < WP) {
+        } else if (v_kg < 4) {
             if (tree)
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if (clean(j * DV, DV)) atomicOr(&bad[step % 3][v_rec], 1u << (4 * v_kg + (j < 4 ? j : 12 + j)));
+                    if (clean(j * DV, DV)) atomicOr(&bad[step % 3], 1u << (4 * v_kg + (j < 4 ? j : 12 + j)));
 #pragma unroll
             for (int i = 0; i < DV; ++i) {
                 const int d = v_d + i, dt = d >> 4;
-                unsigned char* to = buf + v_rec * REC + kKeys + dt * kFrag + 16 * v_entry(d & 15, dt, v_kg);
+                unsigned char* to = buf + kKeys + dt * kFrag + 16 * v_entry(d & 15, dt, v_kg);
                 if constexpr (kPair) {
                     h8_t hi, lo;
                     split8([&](int j) { return __uint_as_float(raw[j * DV + i]); }, pow2f(ev), hi, lo);
@@ -269,8 +265,8 @@ __global__ __launch_bounds__(64 * WR * WP) void k_tree_attn(const TreeAttnArgs a
 
 #pragma unroll
     for (int i = 0; i < kWords; ++i) raw[i] = 0;
-    if (tid < 3 * WP) bad[tid / WP][tid % WP] = 0;
-    places(BN - 1);
+    if (tid < 3) bad[tid] = 0;
+    places(kRec - 1);
     load(0);
 
     // ---- the wave's queries: lane l holds row l % 16 of each subtile, dims 32 c + 8 (l / 16) ..
@@ -279,7 +275,7 @@ __global__ __launch_bounds__(64 * WR * WP) void k_tree_attn(const TreeAttnArgs a
     int row[QS];
 #pragma unroll
     for (int qs = 0; qs < QS; ++qs) {
-        row[qs] = (blk * WR + wr) * 16 * QS + 16 * qs + l16;
+        row[qs] = (blk * NW + wave) * 16 * QS + 16 * qs + l16;
         const int r = min(row[qs], rows - 1);
         const float* qr = a.q + (int64_t)(r / rep) * a.ldq + (int64_t)(g * rep + r % rep) * hd;
         float v[NC][8], m = 0.0f;
@@ -323,8 +319,8 @@ __global__ __launch_bounds__(64 * WR * WP) void k_tree_attn(const TreeAttnArgs a
 
     // ---- one record: ke and ve its scales; TREE: it reaches into the tree
     auto record = [&](auto TREE, int step, int ke, int ve) __attribute__((always_inline)) {
-        const unsigned char* rec = lds + ((step & 1) * WP + wp) * REC;
-        const int p = BN * (u0 + step) + kRec * wp;
+        const unsigned char* rec = lds + (step & 1) * REC;
+        const int p = kRec * (u0 + step);
         f4_t s[QS][2];
 #pragma unroll
         for (int qs = 0; qs < QS; ++qs) s[qs][0] = s[qs][1] = (f4_t){0.0f, 0.0f, 0.0f, 0.0f};
@@ -353,7 +349,7 @@ __global__ __launch_bounds__(64 * WR * WP) void k_tree_attn(const TreeAttnArgs a
         uint32_t bits[QS], odd = 0;
         if constexpr (TREE()) {
             // bit b: the row sees position p + b
-            odd = bad[step % 3][wp];
+            odd = bad[step % 3];
             const int off = p - a.n_past, left = end - p;
 #pragma unroll
             for (int qs = 0; qs < QS; ++qs) {
@@ -449,62 +445,24 @@ __global__ __launch_bounds__(64 * WR * WP) void k_tree_attn(const TreeAttnArgs a
             scales(t + 1);
             store(t + 1);
         }
-        if (tid < WP) bad[(t + 2) % 3][tid] = 0;
+        if (tid == 0) bad[(t + 2) % 3] = 0;
         if (t + 2 < steps) load(t + 2);
-        if (!TREE() || BN * (u0 + t) + kRec * wp < end) record(TREE, t, ke, ve);
+        record(TREE, t, ke, ve);
         ke = ek;
         ve = ev;
         if (t + 2 < steps) publish(t + 2);
         if (t + 1 < steps) __syncthreads();
     };
-    const int plain = max(0, min(steps, a.n_past / BN - u0));  // steps below n_past
+    const int plain = max(0, min(steps, a.n_past / kRec - u0));  // steps below n_past
     int t = 0;
     for (; t < plain; ++t) step(std::false_type(), t);
     for (; t < steps; ++t) step(std::true_type(), t);
 
-    // ---- the WP waves of a row group, then the row's 4 lanes
+    // ---- the row's 4 lanes
 #pragma unroll
-    for (int qs = 0; qs < QS; ++qs)
+    for (int qs = 0; qs < QS; ++qs) {
         l_run[qs] = quad_sum(l_run[qs]);
-    if constexpr (WP > 1) {
-        float* mg = (float*)lds;  // [wp - 1][wr][word][lane]; unit is the same in all waves but in one without records
-        __syncthreads();
-        if (wp > 0) {
-            float* d = mg + (int64_t)((wp - 1) * WR + wr) * kMergeWords * 64 + lane;
-#pragma unroll
-            for (int qs = 0; qs < QS; ++qs) {
-#pragma unroll
-                for (int i = 0; i < 4 * NT; ++i) d[64 * (qs * (4 * NT + 2) + i)] = ldexpf(acc[qs][i >> 2][i & 3], -unit);
-                d[64 * (qs * (4 * NT + 2) + 4 * NT)] = m_run[qs];
-                d[64 * (qs * (4 * NT + 2) + 4 * NT + 1)] = l_run[qs];
-            }
-        }
-        __syncthreads();
-        if (wp > 0) return;
-#pragma unroll
-        for (int qs = 0; qs < QS; ++qs) {
-            float M = m_run[qs];
-            const float* b = mg + (int64_t)wr * kMergeWords * 64 + lane + 64 * qs * (4 * NT + 2);
-            constexpr int kNext = WR * kMergeWords * 64;
-#pragma unroll
-            for (int w = 0; w < WP - 1; ++w) M = fmaxf(M, b[w * kNext + 64 * 4 * NT]);
-            const float ref = M == -INFINITY ? 0.0f : M;
-            const float own = __builtin_amdgcn_exp2f(m_run[qs] - ref);
-            l_run[qs] *= own;
-#pragma unroll
-            for (int i = 0; i < 4 * NT; ++i) acc[qs][i >> 2][i & 3] = ldexpf(acc[qs][i >> 2][i & 3], -unit) * own;
-#pragma unroll
-            for (int w = 0; w < WP - 1; ++w) {
-                const float f = __builtin_amdgcn_exp2f(b[w * kNext + 64 * 4 * NT] - ref);
-                l_run[qs] = fmaf(f, b[w * kNext + 64 * (4 * NT + 1)], l_run[qs]);
-#pragma unroll
-                for (int i = 0; i < 4 * NT; ++i) acc[qs][i >> 2][i & 3] = fmaf(f, b[w * kNext + 64 * i], acc[qs][i >> 2][i & 3]);
-            }
-            m_run[qs] = M;
-        }
-    } else if constexpr (kPair) {
-#pragma unroll
-        for (int qs = 0; qs < QS; ++qs)
+        if constexpr (kPair)
 #pragma unroll
             for (int i = 0; i < 4 * NT; ++i) acc[qs][i >> 2][i & 3] = ldexpf(acc[qs][i >> 2][i & 3], -unit);
     }
@@ -622,45 +580,43 @@ namespace {
 
 // Rows of a workgroup, positions of a step and splits for a call. See launch_tree_attn.
 struct TreePlan {
-    int hp, bm, bn, blocks, splits;
+    int hp, bm, blocks, splits;
 };
 
 TreePlan tree_plan(int n_tree, int H, int G, int hd, int n_past) {
     TreePlan p{};
     const int rows = n_tree * (H / G);
     p.hp = hd <= 64 ? 64 : (hd <= 128 ? 128 : 256);
-    p.bn = kRec;
-    p.bm = p.hp == 256 || rows <= 64 ? 64 : (rows <= 256 ? 128 : 256);
+    // Workgroups of 256 rows (head sizes up to 128) read keys and values fewest times and run two row subtiles on
+    // every fragment, but fill the chip only where there is enough (more than 128 rows): 16 steps for each of 256 workgroups. Below that,
+    // 64 rows and about two workgroups a CU. (64 queries of 64 heads of 128 over 32,768 fp16 positions: 178 us, by
+    // 64 rows 213; of 32 heads of 64 over 8,191: 31.0 and 29.3.)
+    const int64_t units = ((int64_t)n_past + n_tree + kRec - 1) / kRec;
+    const bool big = p.hp <= 128 && rows > 128 && (int64_t)G * ((rows + 255) / 256) * units >= 16 * 256;
+    p.bm = big ? 256 : 64;
     p.blocks = (rows + p.bm - 1) / p.bm;
-    const int64_t units = ((int64_t)n_past + n_tree + p.bn - 1) / p.bn;
-    const int64_t want = std::max<int64_t>(1, 256 / ((int64_t)G * p.blocks));
-    const int64_t per = (units + std::min(units, want) - 1) / std::min(units, want);
+    const int64_t want = std::min(units, std::max<int64_t>(1, (big ? 256 : 512) / ((int64_t)G * p.blocks)));
+    const int64_t per = (units + want - 1) / want;
     p.splits = (int)((units + per - 1) / per);
     return p;
 }
 
-template <class T, int HP, int WR, int WP, int QS>
+template <class T, int HP, int NW, int QS>
 hipError_t launch_tree(const TreeAttnArgs& a, const TreePlan& p, hipStream_t st) {
-    const dim3 grid((unsigned)(a.G * p.splits * p.blocks)), block(64 * WR * WP);
-    if (p.bm != 16 * QS * WR || p.bn != kRec * WP || p.hp != HP) return hipErrorInvalidValue;
+    static_assert(HP == 256 || NW * QS == 4 || NW * QS == 16, "the plan's rows");
+    const dim3 grid((unsigned)(a.G * p.splits * p.blocks)), block(64 * NW);
     if (a.hd == HP)
-        hipLaunchKernelGGL((k_tree_attn<T, HP, WR, WP, QS, true>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((k_tree_attn<T, HP, NW, QS, true>), grid, block, 0, st, a);
     else
-        hipLaunchKernelGGL((k_tree_attn<T, HP, WR, WP, QS, false>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((k_tree_attn<T, HP, NW, QS, false>), grid, block, 0, st, a);
     return hipGetLastError();
 }
 
 template <class T>
 hipError_t launch_tree_type(const TreeAttnArgs& a, const TreePlan& p, hipStream_t st) {
-    if (p.hp == 256) return launch_tree<T, 256, 4, 1, 1>(a, p, st);
-    if (p.hp == 128) {
-        if (p.bm == 64) return launch_tree<T, 128, 4, 1, 1>(a, p, st);
-        if (p.bm == 128) return launch_tree<T, 128, 8, 1, 1>(a, p, st);
-        return launch_tree<T, 128, 8, 1, 2>(a, p, st);
-    }
-    if (p.bm == 64) return launch_tree<T, 64, 4, 1, 1>(a, p, st);
-    if (p.bm == 128) return launch_tree<T, 64, 8, 1, 1>(a, p, st);
-    return launch_tree<T, 64, 8, 1, 2>(a, p, st);
+    if (p.hp == 256) return launch_tree<T, 256, 4, 1>(a, p, st);
+    if (p.hp == 128) return p.bm == 64 ? launch_tree<T, 128, 4, 1>(a, p, st) : launch_tree<T, 128, 8, 2>(a, p, st);
+    return p.bm == 64 ? launch_tree<T, 64, 4, 1>(a, p, st) : launch_tree<T, 64, 8, 2>(a, p, st);
 }
 
 }  // namespace

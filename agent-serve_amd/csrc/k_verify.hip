@@ -116,16 +116,83 @@ __device__ __forceinline__ double prob(const VerRow& r, float l, int x, double c
     return kept(r, l, x) ? weight(l, r.mx, c) * r.inv_z : 0.0;
 }
 
+// Folds and scans over a wave without LDS round trips: lane permutes within 16 lanes (DPP), then swaps of rows of
+// 16 and of halves. Partners fold the same two values, so every lane ends with the same bits.
+template <int CTRL, class T>
+__device__ __forceinline__ T dpp_of(T v) {
+    constexpr int kWords = sizeof(T) / 4;
+    int w[kWords];
+    __builtin_memcpy(w, &v, sizeof(T));
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = __builtin_amdgcn_update_dpp(0, w[i], CTRL, 0xF, 0xF, false);
+    __builtin_memcpy(&v, w, sizeof(T));
+    return v;
+}
+template <class T, class F>
+__device__ __forceinline__ T wave_fold(T v, F op) {
+    v = op(v, dpp_of<kDppXor1>(v));
+    v = op(v, dpp_of<kDppXor2>(v));
+    v = op(v, dpp_of<kDppHalfMirror>(v));
+    v = op(v, dpp_of<kDppMirror>(v));
+    constexpr int kWords = sizeof(T) / 4;
+    uint32_t w[kWords], x[kWords], y[kWords];
+    __builtin_memcpy(w, &v, sizeof(T));
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+        const auto p = __builtin_amdgcn_permlane16_swap(w[i], w[i], false, false);
+        x[i] = p[0];
+        y[i] = p[1];
+    }
+    T a, b;
+    __builtin_memcpy(&a, x, sizeof(T));
+    __builtin_memcpy(&b, y, sizeof(T));
+    v = op(a, b);
+    __builtin_memcpy(w, &v, sizeof(T));
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+        const auto p = __builtin_amdgcn_permlane32_swap(w[i], w[i], false, false);
+        x[i] = p[0];
+        y[i] = p[1];
+    }
+    __builtin_memcpy(&a, x, sizeof(T));
+    __builtin_memcpy(&b, y, sizeof(T));
+    return op(a, b);
+}
+// A 64-bit value of lane i, uniform.
+template <class T>
+__device__ __forceinline__ T lane_value(T v, int i) {
+    static_assert(sizeof(T) == 8, "two words");
+    int w[2];
+    __builtin_memcpy(w, &v, 8);
+    w[0] = __builtin_amdgcn_readlane(w[0], i);
+    w[1] = __builtin_amdgcn_readlane(w[1], i);
+    __builtin_memcpy(&v, w, 8);
+    return v;
+}
+// The sum of the lanes up to this one.
+template <class T>
+__device__ __forceinline__ T wave_scan(T v) {
+    v += dpp_of<0x111>(v);  // row_shr: the lane 1, 2, 4, 8 below in the row of 16, or 0
+    v += dpp_of<0x112>(v);
+    v += dpp_of<0x114>(v);
+    v += dpp_of<0x118>(v);
+    const T r0 = lane_value(v, 15), r1 = r0 + lane_value(v, 31), r2 = r1 + lane_value(v, 47);
+    const int row = (int)(threadIdx.x & 63) >> 4;
+    return row == 0 ? v : v + (row == 1 ? r0 : (row == 2 ? r1 : r2));
+}
 // Folds over the workgroup; every thread gets the result. red: a word for each wave.
 template <class T, class F>
 __device__ __forceinline__ T block_fold(T v, u64_t* red, F op) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o));
+    v = wave_fold(v, op);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) ((T*)red)[threadIdx.x >> 6] = v;
     __syncthreads();
     v = ((T*)red)[0];
-    for (int w = 1; w < (int)(blockDim.x >> 6); ++w) v = op(v, ((T*)red)[w]);
+#pragma unroll
+    for (int w = 1; w < kVerWaves; ++w) {
+        if (w >= (int)(blockDim.x >> 6)) break;
+        v = op(v, ((T*)red)[w]);
+    }
     return v;
 }
 __device__ __forceinline__ double block_sum(double v, u64_t* red) {
@@ -220,6 +287,14 @@ __global__ __launch_bounds__(kBlock) void k_ver_chunks(const VerifyArgs a, const
     if (threadIdx.x == 0) wk.chunks[(int64_t)row * wk.n_chunks + blockIdx.x] = {sum, mx, mn, arg};
 }
 
+__device__ __forceinline__ double row_sum(double v) {  // over 16 lanes
+    v += dpp_of<kDppXor1>(v);
+    v += dpp_of<kDppXor2>(v);
+    v += dpp_of<kDppHalfMirror>(v);
+    v += dpp_of<kDppMirror>(v);
+    return v;
+}
+
 // A row from its chunks, by each 16 lanes of a wave that ask for one (all of them get it).
 __device__ __forceinline__ VerRow row_of_chunks(const VerifyArgs& a, const VerWork& wk, int row) {
     const int l16 = threadIdx.x & 15;
@@ -238,8 +313,10 @@ __device__ __forceinline__ VerRow row_of_chunks(const VerifyArgs& a, const VerWo
         if (16 * k >= wk.n_chunks) break;
         best = max(best, argmax_key(v[k].mx, v[k].arg));
     }
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) best = max(best, (u64_t)__shfl_xor(best, o));
+    best = max(best, dpp_of<kDppXor1>(best));
+    best = max(best, dpp_of<kDppXor2>(best));
+    best = max(best, dpp_of<kDppHalfMirror>(best));
+    best = max(best, dpp_of<kDppMirror>(best));
     VerRow r;
     r.arg = (int32_t)(0xFFFFFFFFu - (uint32_t)best);
     const uint32_t key = (uint32_t)(best >> 32);
@@ -258,8 +335,7 @@ __device__ __forceinline__ VerRow row_of_chunks(const VerifyArgs& a, const VerWo
             if (16 * k >= wk.n_chunks) break;
             if (l16 + 16 * k < wk.n_chunks && v[k].sum > 0.0) z += v[k].sum * weight(v[k].mx, r.mx, c);
         }
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) z += __shfl_xor(z, o);
+        z = row_sum(z);
         r.z = z;
         r.inv_z = z > 0.0 ? 1.0 / z : 0.0;
     }
@@ -312,12 +388,7 @@ __device__ __forceinline__ bool last_of(uint32_t* count, int n, int* sh) {
 // bin and the mass above it. red: a word for each wave.
 __device__ __forceinline__ void find_bin(u64_t mass, u64_t before, u64_t target, u64_t* red, int* out_bin, u64_t* out_before) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    u64_t run = mass;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const u64_t up = __shfl_up(run, o);
-        if (lane >= o) run += up;
-    }
+    const u64_t run = wave_scan(mass);
     __syncthreads();
     if (lane == 63) red[wave] = run;
     __syncthreads();
@@ -356,8 +427,7 @@ __global__ __launch_bounds__(kCutThreads) void k_ver_bins(const VerifyArgs a, co
         else
             atomicAdd(&mass[b], w);
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) low += __shfl_xor(low, o);
+    low = wave_fold(low, [](u64_t x, u64_t y) { return x + y; });
     if ((tid & 63) == 0 && low) atomicAdd(&mass[kBins - 1], low);
     __syncthreads();
     u64_t* part = wk.mass + (int64_t)row * wk.n_cuts * kBins;
@@ -647,13 +717,7 @@ __device__ int draw(const Left& f, int vocab, const double* sums, int n_chunks, 
     // every wave scans the chunks' sums: lane i holds those of 2 i and 2 i + 1
     static_assert(kMaxChunks <= 128, "two chunks a lane");
     const double s0 = 2 * lane < n_chunks ? sums[2 * lane] : 0.0, s1 = 2 * lane + 1 < n_chunks ? sums[2 * lane + 1] : 0.0;
-    double run = s0 + s1;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double x = __shfl_up(run, o);
-        if (lane >= o) run += x;
-    }
-    const double total = __shfl(run, 63);
+    const double run = wave_scan(s0 + s1), total = lane_value(run, 63);
     if (!(total > 0.0)) return -1;
     const double target = u * total, b1 = run - s1;  // the sum up to the lane's second chunk
     // the first chunk with anything left whose running sum passes the target, else the last with anything left
@@ -667,7 +731,8 @@ __device__ int draw(const Left& f, int vocab, const double* sums, int n_chunks, 
         const int i = 63 - __clzll(any0 | any1);
         chunk = 2 * i + (any1 >> i & 1 ? 1 : 0);
     }
-    const double before = __shfl(chunk & 1 ? b1 : b1 - s0, chunk >> 1);
+    chunk = __builtin_amdgcn_readfirstlane(chunk);
+    const double before = lane_value(chunk & 1 ? b1 : b1 - s0, chunk >> 1);
     const int x0 = chunk * kChunk, n = min(kChunk, vocab - x0), at = E * tid;
     float l[E], q[E];
     double w[E], mine = 0.0;
@@ -678,12 +743,7 @@ __device__ int draw(const Left& f, int vocab, const double* sums, int n_chunks, 
         w[k] = kept(f.r, l[k], x0 + at + k) ? f.of_kept(l[k], f.q ? q[k] : 0.0f, x0 + at + k) : 0.0;
         mine += w[k];
     }
-    double up = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double x = __shfl_up(up, o);
-        if (lane >= o) up += x;
-    }
+    const double up = wave_scan(mine);
     if (lane == 63) ((double*)red)[wave] = up;
     if (tid == 0) {
         sh[0] = INT_MAX;
@@ -691,7 +751,8 @@ __device__ int draw(const Left& f, int vocab, const double* sums, int n_chunks, 
     }
     __syncthreads();
     double cum = before + up - mine;
-    for (int i = 0; i < wave; ++i) cum += ((double*)red)[i];
+#pragma unroll
+    for (int i = 0; i < kVerWaves; ++i) cum += i < wave ? ((double*)red)[i] : 0.0;
     int hit = INT_MAX, last = -1;
 #pragma unroll
     for (int k = 0; k < E; ++k) {
@@ -701,15 +762,10 @@ __device__ int draw(const Left& f, int vocab, const double* sums, int n_chunks, 
             last = at + k;
         }
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        hit = min(hit, __shfl_xor(hit, o));
-        last = max(last, __shfl_xor(last, o));
-    }
-    if (lane == 0) {
-        atomicMin(&sh[0], hit);
-        atomicMax(&sh[1], last);
-    }
+    // a wave's first hit is its first such lane's, its last token its last such lane's
+    const u64_t hits = __ballot(hit != INT_MAX), lasts = __ballot(last >= 0);
+    if (hits && lane == __ffsll((unsigned long long)hits) - 1) atomicMin(&sh[0], hit);
+    if (lasts && lane == 63 - __clzll(lasts)) atomicMax(&sh[1], last);
     __syncthreads();
     const int tok = sh[0] == INT_MAX ? sh[1] : sh[0];  // past the sums' rounding: the last token that is left
 #pragma unroll
@@ -763,8 +819,7 @@ __global__ __launch_bounds__(kVerThreads) void k_ver_walk(const VerifyArgs a, co
         if (sampled) {
             double s = 0.0;
             for (int k = tid & 15; k < wk.n_chunks; k += 16) s += wk.round[(int64_t)i * wk.n_chunks + k];
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o);
+            s = row_sum(s);
             if ((tid & 15) == 0) s1[i] = s;  // of rows with fewer than two children: not written, and not used
         }
     }
