@@ -104,8 +104,7 @@ __global__ __launch_bounds__(64 * NW) void k_tree_attn(const TreeAttnArgs a) {
     // Keys: a wave's unit is 16 positions x 32 dims of a fragment, lane = (position lane / 4, 8 dims from
     // 8 (lane % 4)), which is entry 16 (lane % 4) + (position ^ 2 (lane % 4)). Values: a thread holds the
     // 8 positions of a key group (4 kg + 0..3 and 16 + 4 kg + 0..3, as the weights lie in the lanes) of
-    // DV dims. A step's base is uniform and a thread's places in it are 32-bit offsets, found again for a
-    // step past the end, which repeats the last row.
+    // DV dims.
     constexpr int kHalf = NW / 2;
     const bool key_wave = wave < kHalf;
     const int tv = tid - 64 * kHalf;  // value threads
@@ -118,23 +117,10 @@ __global__ __launch_bounds__(64 * NW) void k_tree_attn(const TreeAttnArgs a) {
         else
             return h2f(i & 1 ? raw[i / 2] >> 16 : raw[i / 2] & 0xFFFFu);
     };
-    auto key_dim = [&](int u) { return 32 * ((wave * kUnits + u) % NC) + 8 * (lane & 3); };
-    uint32_t off[kUnits > 8 ? kUnits : 8];
-    auto places = [&](int most) __attribute__((always_inline)) {  // most: the step's last position
-        if (key_wave) {
-#pragma unroll
-            for (int u = 0; u < kUnits; ++u) {
-                const int pos = min(16 * ((wave * kUnits + u) / NC) + (lane >> 2), most), d = key_dim(u);
-                off[u] = (uint32_t)(pos * stride + (EXACT || d < hd ? d : 0)) * kE;
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int pos = min(4 * v_kg + (j < 4 ? j : 12 + j), most);
-                off[j] = (uint32_t)(pos * stride + (EXACT || v_d < hd ? v_d : 0)) * kE;
-            }
-        }
-    };
+    // The thread's first place in a step; its others are uniform distances away. Dims past the head's are loaded
+    // from dim 0 and zeros take their place. Every offset is from a row's start and not negative.
+    const int my_pos = key_wave ? lane >> 2 : 4 * v_kg, my_dim = key_wave ? 8 * (lane & 3) : v_d;
+    const int row_bytes = stride * kE;
     auto words = [&](const char* q, uint32_t* to, auto n) __attribute__((always_inline)) {
         if constexpr (n() >= 4) {
 #pragma unroll
@@ -149,25 +135,38 @@ __global__ __launch_bounds__(64 * NW) void k_tree_attn(const TreeAttnArgs a) {
             to[0] = *(const TF_GLOBAL uint32_t*)q;
         }
     };
-    auto load = [&](int step) __attribute__((always_inline)) {
-        const int p = kRec * (u0 + step);
-        if (p + kRec > end) places(end - 1 - p);
-        const char* at = src + (int64_t)p * stride * kE;
+    auto load_as = [&](auto FULL, int step) __attribute__((always_inline)) {
+        const int p = kRec * (u0 + step), last = end - 1 - p;  // last: the end's position in the step
+        const char* at = src + (int64_t)p * row_bytes;
+        // place (row, dim) from the thread's first; past the end the last row repeats
+        const uint32_t mine = (uint32_t)(my_pos * row_bytes + my_dim * kE);
+        auto place = [&](int row, int dim) __attribute__((always_inline)) -> const char* {
+            if constexpr (FULL() && EXACT) return at + (row * row_bytes + dim * kE) + mine;
+            const int d = EXACT || my_dim + dim < hd ? my_dim + dim : 0;
+            return at + (uint32_t)(min(my_pos + row, last) * row_bytes + d * kE);
+        };
         if (key_wave) {
 #pragma unroll
             for (int u = 0; u < kUnits; ++u) {
-                words(at + off[u], raw + u * 2 * kE, std::integral_constant<int, 2 * kE>());
-                if (!EXACT && key_dim(u) >= hd)
+                const int wu = wave * kUnits + u, dim = 32 * (wu % NC);  // (half, chunk)
+                words(place(16 * (wu / NC), dim), raw + u * 2 * kE, std::integral_constant<int, 2 * kE>());
+                if (!EXACT && my_dim + dim >= hd)
 #pragma unroll
                     for (int i = 0; i < 2 * kE; ++i) raw[u * 2 * kE + i] = 0;
             }
         } else if (v_kg < 4) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) words(at + off[j], raw + j * DV * kE / 4, std::integral_constant<int, DV * kE / 4>());
+            for (int j = 0; j < 8; ++j) words(place(j < 4 ? j : 12 + j, 0), raw + j * DV * kE / 4, std::integral_constant<int, DV * kE / 4>());
             if (!EXACT && v_d >= hd)
 #pragma unroll
                 for (int i = 0; i < 2 * DV * kE; ++i) raw[i] = 0;
         }
+    };
+    auto load = [&](int step) __attribute__((always_inline)) {
+        if (kRec * (u0 + step + 1) <= end)
+            load_as(std::true_type(), step);
+        else
+            load_as(std::false_type(), step);
     };
     // the largest finite magnitude of this wave's elements, for their scale
     auto publish = [&](int step) __attribute__((always_inline)) {
@@ -266,7 +265,6 @@ __global__ __launch_bounds__(64 * NW) void k_tree_attn(const TreeAttnArgs a) {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) raw[i] = 0;
     if (tid < 3) bad[tid] = 0;
-    places(kRec - 1);
     load(0);
 
     // ---- the wave's queries: lane l holds row l % 16 of each subtile, dims 32 c + 8 (l / 16) ..
