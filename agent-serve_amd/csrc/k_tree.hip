@@ -10,8 +10,9 @@
 // between. fp32 operands enter as fp16 pairs hi + lo (22 significant bits): x y = hi_x hi_y +
 // hi_x lo_y + lo_x hi_y, the rest being 2^-22 of the product; fp16 caches are operands as they
 // are, so only q and p are pairs. Numbers are scaled by powers of two, exactly taken out again:
-//   a query row by its largest element; a tile's keys by the tile's largest, its values likewise
-//   (both in [2^14, 2^15): fp16 pairs hold 22 bits down to 2^-18 of that, and 2^-40 of it below);
+//   a query row by its largest element; the 8 or 16 keys that a wave loads by their largest, the values
+//   that it does likewise (all in [2^14, 2^15): fp16 pairs hold 22 bits down to 2^-18 of that, and 2^-40 of
+//   it below);
 //   a weight by 2^14, so that weights down to 2^-18 of the row's largest keep 22 bits.
 // The softmax's running reference is the score's maximum in units of log2, rounded up to a whole
 // number: rescaling by 2^(old - new) is exact, and it is needed only when the maximum passes one.
@@ -19,7 +20,7 @@
 // A workgroup of NW waves takes 16 QS rows of one kv head a wave and one split of the positions, 32 at a
 // time (a step): the step's keys and values lie in LDS in fragment order (a record), and every wave runs its
 // rows over them. Half of the threads load, scale and store keys, half values, one step ahead of the
-// products; loads are two steps ahead. Splits are merged by k_tree_merge; one split writes the output itself.
+// products; the next step's loads are under way meanwhile. Splits are merged by k_tree_merge; one split writes the output itself.
 #include <algorithm>
 #include <type_traits>
 
@@ -77,7 +78,8 @@ template <class T, int HP, int NW, int QS, bool EXACT>
 __global__ __launch_bounds__(64 * NW) void k_tree_attn(const TreeAttnArgs a) {
     constexpr bool kPair = sizeof(T) == 4;
     constexpr int NC = HP / 32, NT = HP / 16, kE = (int)sizeof(T);
-    constexpr int kUnits = HP / NW / 8;  // units of 8 key elements a thread loads per step
+    // Keys: a wave takes kWaveKeys positions of a step, kLanes lanes a position, 64 / kLanes positions a unit.
+    constexpr int kHalf = NW / 2, kWaveKeys = kRec / kHalf, kLanes = HP / 8, kUnits = kWaveKeys * kLanes / 64;
     // dims of 8 values each a thread loads per step: at least a word of them (then some threads load none)
     constexpr int DV = HP / NW / 8 > 4 / kE ? HP / NW / 8 : 4 / kE;
     constexpr int kWords = (kUnits > DV ? kUnits : DV) * 8 * kE / 4;
@@ -86,7 +88,7 @@ __global__ __launch_bounds__(64 * NW) void k_tree_attn(const TreeAttnArgs a) {
     constexpr int kBufs = 2;
     static_assert(NW % 2 == 0 && HP / NW >= 8, "half of the waves load keys, half values");
     __shared__ __align__(16) unsigned char lds[kBufs * REC];
-    __shared__ float amax[2][NW];
+    __shared__ int scale_of[2][NW];  // the exponents of a step's key waves and value waves, by step mod 2
     __shared__ uint32_t bad[3];  // positions of a record with an infinity or NaN, by step mod 3
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -101,11 +103,10 @@ __global__ __launch_bounds__(64 * NW) void k_tree_attn(const TreeAttnArgs a) {
     const int64_t base = kv_offset(a.layout, a.G, a.max_seq, hd, g, 0);
 
     // ---- loads
-    // Keys: a wave's unit is 16 positions x 32 dims of a fragment, lane = (position lane / 4, 8 dims from
-    // 8 (lane % 4)), which is entry 16 (lane % 4) + (position ^ 2 (lane % 4)). Values: a thread holds the
-    // 8 positions of a key group (4 kg + 0..3 and 16 + 4 kg + 0..3, as the weights lie in the lanes) of
-    // DV dims.
-    constexpr int kHalf = NW / 2;
+    // Keys: lane = (position lane / kLanes of a unit, 8 dims); they are entry 16 ch + (position ^ 2 ch ^ c mod 2)
+    // of the fragment of their half and chunk c (ch: their place among its 4 times 8 dims), which leaves 8
+    // consecutive lanes on 8 different 16-byte banks. Values: a thread holds the 8 positions of a key group
+    // (4 kg + 0..3 and 16 + 4 kg + 0..3, as the weights lie in the lanes) of DV dims.
     const bool key_wave = wave < kHalf;
     const int tv = tid - 64 * kHalf;  // value threads
     const int v_d = DV * (tv % (HP / DV)), v_kg = tv / (HP / DV);
@@ -119,7 +120,8 @@ __global__ __launch_bounds__(64 * NW) void k_tree_attn(const TreeAttnArgs a) {
     };
     // The thread's first place in a step; its others are uniform distances away. Dims past the head's are loaded
     // from dim 0 and zeros take their place. Every offset is from a row's start and not negative.
-    const int my_pos = key_wave ? lane >> 2 : 4 * v_kg, my_dim = key_wave ? 8 * (lane & 3) : v_d;
+    const int k_pos = wave * kWaveKeys + lane / kLanes;  // its unit 0's position
+    const int my_pos = key_wave ? k_pos : 4 * v_kg, my_dim = key_wave ? 8 * (lane % kLanes) : v_d;
     const int row_bytes = stride * kE;
     auto words = [&](const char* q, uint32_t* to, auto n) __attribute__((always_inline)) {
         if constexpr (n() >= 4) {
@@ -138,29 +140,23 @@ __global__ __launch_bounds__(64 * NW) void k_tree_attn(const TreeAttnArgs a) {
     auto load_as = [&](auto FULL, int step) __attribute__((always_inline)) {
         const int p = kRec * (u0 + step), last = end - 1 - p;  // last: the end's position in the step
         const char* at = src + (int64_t)p * row_bytes;
-        // place (row, dim) from the thread's first; past the end the last row repeats
-        const uint32_t mine = (uint32_t)(my_pos * row_bytes + my_dim * kE);
-        auto place = [&](int row, int dim) __attribute__((always_inline)) -> const char* {
-            if constexpr (FULL() && EXACT) return at + (row * row_bytes + dim * kE) + mine;
-            const int d = EXACT || my_dim + dim < hd ? my_dim + dim : 0;
-            return at + (uint32_t)(min(my_pos + row, last) * row_bytes + d * kE);
+        // place `row` rows below the thread's first; past the end the last row repeats
+        const int dim = EXACT || my_dim < hd ? my_dim : 0;
+        const uint32_t mine = (uint32_t)(my_pos * row_bytes + dim * kE);
+        auto place = [&](int row) __attribute__((always_inline)) -> const char* {
+            if constexpr (FULL()) return at + row * row_bytes + mine;
+            return at + (uint32_t)(min(my_pos + row, last) * row_bytes + dim * kE);
         };
         if (key_wave) {
 #pragma unroll
-            for (int u = 0; u < kUnits; ++u) {
-                const int wu = wave * kUnits + u, dim = 32 * (wu % NC);  // (half, chunk)
-                words(place(16 * (wu / NC), dim), raw + u * 2 * kE, std::integral_constant<int, 2 * kE>());
-                if (!EXACT && my_dim + dim >= hd)
-#pragma unroll
-                    for (int i = 0; i < 2 * kE; ++i) raw[u * 2 * kE + i] = 0;
-            }
+            for (int u = 0; u < kUnits; ++u) words(place(u * (64 / kLanes)), raw + u * 2 * kE, std::integral_constant<int, 2 * kE>());
         } else if (v_kg < 4) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) words(place(j < 4 ? j : 12 + j, 0), raw + j * DV * kE / 4, std::integral_constant<int, DV * kE / 4>());
-            if (!EXACT && v_d >= hd)
-#pragma unroll
-                for (int i = 0; i < 2 * DV * kE; ++i) raw[i] = 0;
+            for (int j = 0; j < 8; ++j) words(place(j < 4 ? j : 12 + j), raw + j * DV * kE / 4, std::integral_constant<int, DV * kE / 4>());
         }
+        if (!EXACT && my_dim >= hd)
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) raw[i] = 0;
     };
     auto load = [&](int step) __attribute__((always_inline)) {
         if (kRec * (u0 + step + 1) <= end)
@@ -168,40 +164,20 @@ __global__ __launch_bounds__(64 * NW) void k_tree_attn(const TreeAttnArgs a) {
         else
             load_as(std::false_type(), step);
     };
-    // the largest finite magnitude of this wave's elements, for their scale
-    auto publish = [&](int step) __attribute__((always_inline)) {
-        if constexpr (kPair) {
-            float m = 0.0f;
+    // the power of two that this wave's elements are scaled by, from the largest finite one
+    auto scale = [&]() __attribute__((always_inline)) -> int {
+        float m = 0.0f;
 #pragma unroll
-            for (int i = 0; i < kWords; ++i) m = fmaxf(m, fabsf(__uint_as_float(raw[i])));
-            if (!(m < INFINITY)) {
-                m = 0.0f;
+        for (int i = 0; i < kWords; ++i) m = fmaxf(m, fabsf(__uint_as_float(raw[i])));
+        if (!(m < INFINITY)) {
+            m = 0.0f;
 #pragma unroll
-                for (int i = 0; i < kWords; ++i) {
-                    const float x = fabsf(__uint_as_float(raw[i]));
-                    if (x < INFINITY) m = fmaxf(m, x);
-                }
+            for (int i = 0; i < kWords; ++i) {
+                const float x = fabsf(__uint_as_float(raw[i]));
+                if (x < INFINITY) m = fmaxf(m, x);
             }
-            m = wave_max(m);
-            if (lane == 0) amax[step & 1][wave] = m;
         }
-    };
-    // The next step's scales. Values far below earlier ones are not scaled all the way up: their weights
-    // shrink by as much (they go into the same sum), and are to stay in range.
-    constexpr int kMostUp = 30;
-    int ek = 0, ev = 0, ev_min = 126 - kMostUp;
-    auto scales = [&](int step) {
-        if constexpr (kPair) {
-            float mk = 0.0f, mv = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kHalf; ++w) {
-                mk = fmaxf(mk, amax[step & 1][w]);
-                mv = fmaxf(mv, amax[step & 1][kHalf + w]);
-            }
-            ek = __builtin_amdgcn_readfirstlane(scale_exp(mk));
-            ev = min(__builtin_amdgcn_readfirstlane(scale_exp(mv)), ev_min + kMostUp);
-            ev_min = min(ev_min, ev);
-        }
+        return scale_exp(wave_max(m));
     };
     // Infinities and NaN among `n` elements from i are taken out; whether there were any.
     auto clean = [&](int i, int n) __attribute__((always_inline)) {
@@ -222,15 +198,22 @@ __global__ __launch_bounds__(64 * NW) void k_tree_attn(const TreeAttnArgs a) {
     auto store = [&](int step) __attribute__((always_inline)) {
         unsigned char* buf = lds + (step & 1) * REC;
         const bool tree = kRec * (u0 + step + 1) > a.n_past;
+        float sc = 1.0f;
+        if constexpr (kPair) {
+            const int e = scale();
+            sc = pow2f(e);
+            if (lane == 0) scale_of[step & 1][wave] = e;
+        }
         if (key_wave) {
+            const int c = lane % kLanes >> 2, ch = lane & 3;
 #pragma unroll
             for (int u = 0; u < kUnits; ++u) {
-                const int hc = wave * kUnits + u, ch = lane & 3;  // (half, chunk)
-                if (tree && clean(8 * u, 8)) atomicOr(&bad[step % 3], 1u << (16 * (hc / NC) + (lane >> 2)));
-                unsigned char* to = buf + hc * kFrag + 16 * (16 * ch + ((lane >> 2) ^ (2 * ch)));
+                const int pos = k_pos + u * (64 / kLanes);
+                if (tree && clean(8 * u, 8)) atomicOr(&bad[step % 3], 1u << pos);
+                unsigned char* to = buf + ((pos >> 4) * NC + c) * kFrag + 16 * (16 * ch + ((pos & 15) ^ (2 * ch) ^ (c & 1)));
                 if constexpr (kPair) {
                     h8_t hi, lo;
-                    split8([&](int j) { return __uint_as_float(raw[8 * u + j]); }, pow2f(ek), hi, lo);
+                    split8([&](int j) { return __uint_as_float(raw[8 * u + j]); }, sc, hi, lo);
                     *(h8_t*)to = hi;
                     *(h8_t*)(to + 1024) = lo;
                 } else {
@@ -248,7 +231,7 @@ __global__ __launch_bounds__(64 * NW) void k_tree_attn(const TreeAttnArgs a) {
                 unsigned char* to = buf + kKeys + dt * kFrag + 16 * v_entry(d & 15, dt, v_kg);
                 if constexpr (kPair) {
                     h8_t hi, lo;
-                    split8([&](int j) { return __uint_as_float(raw[j * DV + i]); }, pow2f(ev), hi, lo);
+                    split8([&](int j) { return __uint_as_float(raw[j * DV + i]); }, sc, hi, lo);
                     *(h8_t*)to = hi;
                     *(h8_t*)(to + 1024) = lo;
                 } else {
@@ -265,6 +248,7 @@ __global__ __launch_bounds__(64 * NW) void k_tree_attn(const TreeAttnArgs a) {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) raw[i] = 0;
     if (tid < 3) bad[tid] = 0;
+    __syncthreads();  // before store(0) sets bits of it
     load(0);
 
     // ---- the wave's queries: lane l holds row l % 16 of each subtile, dims 32 c + 8 (l / 16) ..
@@ -310,23 +294,24 @@ __global__ __launch_bounds__(64 * NW) void k_tree_attn(const TreeAttnArgs a) {
 #pragma unroll
         for (int d = 0; d < NT; ++d) acc[qs][d] = (f4_t){0.0f, 0.0f, 0.0f, 0.0f};
     }
-    const int k_at = 16 * (16 * gq + (l16 ^ (2 * gq)));
+    const int k_at[2] = {16 * (16 * gq + (l16 ^ (2 * gq))), 16 * (16 * gq + (l16 ^ (2 * gq) ^ 1))};
     int v_at[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) v_at[i] = 16 * v_entry(l16, i, gq);
 
-    // ---- one record: ke and ve its scales; TREE: it reaches into the tree
-    auto record = [&](auto TREE, int step, int ke, int ve) __attribute__((always_inline)) {
+    // ---- one record; TREE: it reaches into the tree
+    auto record = [&](auto TREE, int step) __attribute__((always_inline)) {
         const unsigned char* rec = lds + (step & 1) * REC;
         const int p = kRec * (u0 + step);
         f4_t s[QS][2];
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int qs = 0; qs < QS; ++qs) s[qs][0] = s[qs][1] = (f4_t){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const unsigned char* f = rec + (half * NC + c) * kFrag + k_at;
+                const unsigned char* f = rec + (half * NC + c) * kFrag + k_at[c & 1];
                 const h8_t kh = *(const h8_t*)f;
 #pragma unroll
                 for (int qs = 0; qs < QS; ++qs) s[qs][half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[qs][c], s[qs][half], 0, 0, 0);
@@ -338,6 +323,7 @@ __global__ __launch_bounds__(64 * NW) void k_tree_attn(const TreeAttnArgs a) {
                     for (int qs = 0; qs < QS; ++qs) s[qs][half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[qs][c], s[qs][half], 0, 0, 0);
                 }
             }
+        __builtin_amdgcn_s_setprio(0);
         // the values are read ahead of the softmax, whose branches they would otherwise wait behind
         h8_t vh[NT];
 #pragma unroll
@@ -364,11 +350,19 @@ __global__ __launch_bounds__(64 * NW) void k_tree_attn(const TreeAttnArgs a) {
                 bits[qs] = (uint32_t)x & (left >= 32 ? 0xFFFFFFFFu : (1u << left) - 1);
             }
         }
-        // values smaller than an earlier step's: the weights shrink; larger ones: the output does
-        int e = 0, shift = kWeightExp;
+        // The scales of the lane's keys (its first four positions, its last four) and values, and the output's unit:
+        // the least of the values' scales so far. Values of a greater one have their weights shrunk by as much.
+        int ke[2] = {0, 0}, e = 0;
+        float shrink = 1.0f;
         if constexpr (kPair) {
-            e = min(unit, ve);
-            shift = kWeightExp + e - ve;
+            const int* of = scale_of[step & 1];
+            e = unit;
+#pragma unroll
+            for (int w = 0; w < kHalf; ++w) e = min(e, of[kHalf + w]);
+            e = __builtin_amdgcn_readfirstlane(e);
+            ke[0] = of[4 * gq / kWaveKeys];
+            ke[1] = of[(16 + 4 * gq) / kWaveKeys];
+            shrink = pow2f(max(e - of[kHalf + gq * kHalf / 4], -126));
         }
         const int de = e - unit;
         unit = e;
@@ -377,8 +371,9 @@ __global__ __launch_bounds__(64 * NW) void k_tree_attn(const TreeAttnArgs a) {
         bool scaled = false;
 #pragma unroll
         for (int qs = 0; qs < QS; ++qs) {
-            const float f = fmaxf(kPair ? ldexpf(fq[qs], -ke) : fq[qs], 1e-37f);
-            float x[8], mt = -INFINITY;
+            float f[2], x[8], mt[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int i = 0; i < 2; ++i) f[i] = fmaxf(kPair ? ldexpf(fq[qs], -ke[i]) : fq[qs], 1e-37f);
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] = s[qs][j >> 2][j & 3];
             if constexpr (TREE()) {
@@ -390,20 +385,23 @@ __global__ __launch_bounds__(64 * NW) void k_tree_attn(const TreeAttnArgs a) {
                 }
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) mt = fmaxf(mt, x[j]);
-            mt = quad_max(mt);
-            const float m_new = fmaxf(m_run[qs], ceilf(mt * f));
+            for (int j = 0; j < 8; ++j) mt[j >> 2] = fmaxf(mt[j >> 2], x[j]);
+            const float top = quad_max(kPair ? fmaxf(mt[0] * f[0], mt[1] * f[1]) : fmaxf(mt[0], mt[1]) * f[0]);
+            const float m_new = fmaxf(m_run[qs], ceilf(top));
             const float m_ref = m_new == -INFINITY ? 0.0f : m_new;
             const float alpha = __builtin_amdgcn_exp2f(m_run[qs] - m_ref);
-            const float sh = (float)shift - m_ref;
+            const float sh = (float)kWeightExp - m_ref;
             float ls = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                x[j] = __builtin_amdgcn_exp2f(fmaf(x[j], f, sh));
+                x[j] = __builtin_amdgcn_exp2f(fmaf(x[j], f[kPair ? j >> 2 : 0], sh));
                 ls += x[j];
             }
-            split8([&](int j) { return x[j]; }, ph[qs], pl[qs]);
-            l_run[qs] = fmaf(l_run[qs], alpha, kPair ? ldexpf(ls, -shift) : ls * pow2f(-kWeightExp));
+            if constexpr (kPair)
+                split8([&](int j) { return x[j]; }, shrink, ph[qs], pl[qs]);
+            else
+                split8([&](int j) { return x[j]; }, ph[qs], pl[qs]);
+            l_run[qs] = fmaf(l_run[qs], alpha, ls * pow2f(-kWeightExp));
             m_run[qs] = m_new;
             resc[qs] = kPair ? ldexpf(alpha, de) : alpha;
             scaled = scaled || resc[qs] != 1.0f;
@@ -413,6 +411,7 @@ __global__ __launch_bounds__(64 * NW) void k_tree_attn(const TreeAttnArgs a) {
             for (int qs = 0; qs < QS; ++qs)
 #pragma unroll
                 for (int d = 0; d < NT; ++d) acc[qs][d] = acc[qs][d] * resc[qs];
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int d = 0; d < NT; ++d) {
 #pragma unroll
@@ -425,31 +424,23 @@ __global__ __launch_bounds__(64 * NW) void k_tree_attn(const TreeAttnArgs a) {
                 for (int qs = 0; qs < QS; ++qs) acc[qs][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[qs], acc[qs][d], 0, 0, 0);
             }
         }
+        __builtin_amdgcn_s_setprio(0);
     };
 
-    publish(0);
-    __syncthreads();
-    scales(0);
+    // every wave's LDS writes are done; loads under way stay so, which __syncthreads would wait for
+    auto barrier = [&]() __attribute__((always_inline)) { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
     store(0);
-    int ke = ek, ve = ev;
-    if (steps > 1) {
-        load(1);
-        publish(1);
-    }
-    __syncthreads();
-    // step t: records t are complete, and the loads of t + 1 with their scale
+    if (steps > 1) load(1);
+    barrier();
+    // step t: its record is complete, the loads of t + 1 are there or under way. The next step's stores go first:
+    // the waves leave the barrier together, and those on the vector units keep out of the way of the matrix ones
+    // (after the record 30.0 us instead of 27.7 for 64 queries of 32 heads over 8,191 fp16 positions).
     auto step = [&](auto TREE, int t) __attribute__((always_inline)) {
-        if (t + 1 < steps) {
-            scales(t + 1);
-            store(t + 1);
-        }
+        if (t + 1 < steps) store(t + 1);
         if (tid == 0) bad[(t + 2) % 3] = 0;
         if (t + 2 < steps) load(t + 2);
-        record(TREE, t, ke, ve);
-        ke = ek;
-        ve = ev;
-        if (t + 2 < steps) publish(t + 2);
-        if (t + 1 < steps) __syncthreads();
+        record(TREE, t);
+        if (t + 1 < steps) barrier();
     };
     const int plain = max(0, min(steps, a.n_past / kRec - u0));  // steps below n_past
     int t = 0;
