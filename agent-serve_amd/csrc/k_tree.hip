@@ -594,11 +594,7 @@ template <class T, int HP, int NW, int QS>
 hipError_t launch_tree(const TreeAttnArgs& a, const TreePlan& p, hipStream_t st) {
     static_assert(HP == 256 || NW * QS == 4 || NW * QS == 16, "the plan's rows");
     const dim3 grid((unsigned)(a.G * p.splits * p.blocks)), block(64 * NW);
-    if (a.hd == HP)
-        hipLaunchKernelGGL((k_tree_attn<T, HP, NW, QS, true>), grid, block, 0, st, a);
-    else
-        hipLaunchKernelGGL((k_tree_attn<T, HP, NW, QS, false>), grid, block, 0, st, a);
-    return hipGetLastError();
+    return launch_kernel(a.hd == HP ? k_tree_attn<T, HP, NW, QS, true> : k_tree_attn<T, HP, NW, QS, false>, grid, block, st, a);
 }
 
 template <class T>
@@ -625,14 +621,12 @@ hipError_t launch_tree_attn(const TreeAttnArgs& args, void* ws, hipStream_t st) 
     const hipError_t e = a.kv_type == TF_HIP_TYPE_F32 ? launch_tree_type<float>(a, p, st) : launch_tree_type<_Float16>(a, p, st);
     if (e != hipSuccess || a.S == 1) return e;
     const int tpr = a.S <= 8 ? 64 : kBlock, rows = a.n_tree * a.H, per = kBlock / tpr;
-    hipLaunchKernelGGL(k_tree_merge, dim3((unsigned)((rows + per - 1) / per)), dim3(kBlock), 0, st, a, tpr);
-    return hipGetLastError();
+    return launch_kernel(k_tree_merge, dim3((unsigned)((rows + per - 1) / per)), dim3(kBlock), st, a, tpr);
 }
 
 hipError_t launch_keep_path(const KeepArgs& a, hipStream_t st) {
     const int64_t pieces = (int64_t)a.n_layer * a.G * a.row16;
-    hipLaunchKernelGGL(k_keep_path, dim3((unsigned)((pieces + kBlock - 1) / kBlock), 2), dim3(kBlock), 0, st, a);
-    return hipGetLastError();
+    return launch_kernel(k_keep_path, dim3((unsigned)((pieces + kBlock - 1) / kBlock), 2), dim3(kBlock), st, a);
 }
 
 }  // namespace tfk

@@ -1000,8 +1000,7 @@ hipError_t launch_verify(const VerifyArgs& a, void* ws, hipStream_t st) {
     const bool greedy = a.temperature <= 0.0f, cut = !greedy && a.top_p < 1.0f, sampled = !greedy && a.draft;
     const dim3 grid((unsigned)wk.n_chunks, (unsigned)a.n_tree);
     auto launch = [&](void (*k)(VerifyArgs, VerWork), dim3 g, int threads) {
-        hipLaunchKernelGGL(k, g, dim3(threads), 0, st, a, wk);
-        return hipGetLastError();
+        return launch_kernel(k, g, dim3(threads), st, a, wk);
     };
     hipError_t e = launch(k_ver_chunks, grid, kBlock);
     const dim3 cuts((unsigned)wk.n_cuts, (unsigned)a.n_tree);

@@ -1858,9 +1858,9 @@ struct DeviceScope {
     int before = -1;
     bool ok = false;
     explicit DeviceScope(int device) {
-        if (hipGetDevice(&before) != hipSuccess) return;
-        ok = before == device || hipSetDevice(device) == hipSuccess;
-        if (before == device) before = -1;
+        ok = hipGetDevice(&before) == hipSuccess && (before == device || hipSetDevice(device) == hipSuccess);
+        if (!ok) (void)hipGetLastError();  // reported by this call's status, not to a later one
+        if (!ok || before == device) before = -1;
     }
     ~DeviceScope() {
         if (before >= 0) (void)hipSetDevice(before);

@@ -332,6 +332,20 @@ hipError_t launch_step_split(const StepArgs& a, int n_wg, hipStream_t st);
 hipError_t launch_step_f16(const StepArgs& a, int n_wg, hipStream_t st);
 hipError_t launch_step_q6k(const StepArgs& a, int n_wg, hipStream_t st);
 
+// Launches a kernel and returns this launch's own error: an error that an earlier call of the program left behind
+// is not taken for it, and one of its own is not left behind for a later call to find.
+template <class T>
+struct LaunchArg {
+    typedef T type;
+};
+template <class... A>
+hipError_t launch_kernel(void (*k)(A...), dim3 grid, dim3 block, hipStream_t st, typename LaunchArg<A>::type... a) {
+    void* args[] = {(void*)&a...};
+    const hipError_t e = hipLaunchKernel((const void*)k, grid, block, args, 0, st);
+    if (e != hipSuccess) (void)hipGetLastError();
+    return e;
+}
+
 // ---------------------------------------------------------------- trees of drafted tokens
 constexpr int kTreeMax = TF_HIP_TREE_MAX;
 

@@ -629,3 +629,34 @@ def test_current_device_and_default_stream(lib):
     assert lib.tf_hip_attn_tree(99, F32, x.q.data_ptr(), x.ld, x.k.data_ptr(), x.v.data_ptr(), x.masks.data_ptr(), 3, 4,
                                 2, 64, 20, x.seq, 0, x.out.data_ptr(), x.ld, ws.data_ptr(), ws.numel(), None) == -4
     assert torch.cuda.current_device() == before
+
+
+def test_errors_do_not_outlive_their_call(lib, pkg):
+    """A call that fails (a device that is not there) leaves no error behind for the next call to find, and an
+    error that another call left behind is not taken for this one's."""
+    import ctypes as C
+    x = Attn(4, 2, 64, 3, 20, seed=14)
+    ok = x.check(lib).clone()
+
+    def bad():
+        return lib.tf_hip_attn_tree(99, F32, x.q.data_ptr(), x.ld, x.k.data_ptr(), x.v.data_ptr(), x.masks.data_ptr(), 3,
+                                    4, 2, 64, 20, x.seq, 0, x.out.data_ptr(), x.ld, x.ws.data_ptr(), x.ws.numel(), None)
+    assert bad() == -4
+    rows = np.ones((5, 2, 64), np.float32)
+    assert np.all(pkg.attn_decode(np.ones((4, 64), np.float32), rows, rows, 64, 0) == 1.0)
+    y = Verify(3, 100, seed=15).setup(lib)
+    st = stream()
+    hip = C.CDLL("libamdhip64.so.7")
+    x.out.fill_(NAN)
+    torch.cuda.synchronize()
+    assert hip.hipSetDevice(99) != 0  # leaves the runtime's last error set
+    d = y.d
+    rcs = [lib.tf_hip_attn_tree(0, F32, x.q.data_ptr(), x.ld, x.k.data_ptr(), x.v.data_ptr(), x.masks.data_ptr(), 3, 4, 2,
+                                64, 20, x.seq, 0, x.out.data_ptr(), x.ld, x.ws.data_ptr(), x.ws.numel(), st),
+           lib.tf_hip_verify_tree(0, d["logits"].data_ptr(), 100, 100, d["tokens"].data_ptr(), d["parent"].data_ptr(), 3,
+                                  None, 0, 0.8, 1.0, d["draws"].data_ptr(), d["path"].data_ptr(), d["result"].data_ptr(),
+                                  None, y.ws.data_ptr(), y.ws.numel(), st)]
+    hip.hipGetLastError()
+    assert rcs == [0, 0]
+    torch.cuda.synchronize()
+    assert torch.equal(x.out.view(3, 4, 64).double(), ok)
