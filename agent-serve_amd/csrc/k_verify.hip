@@ -356,22 +356,20 @@ __device__ __forceinline__ void row_range(const VerWork& wk, int row, float& mx,
 // The sums that find where it ends are of 32-bit weights (the last token's place is off only where the
 // running sum comes within 1e-7 of top_p), as integers of 2^-44 of the largest: integers add up to the
 // same in any order, so the atomics do not show. What is kept is summed in 64 bits.
-__device__ __forceinline__ u64_t weight_fix(float l, float mx, float c) {
-    const float w = l == mx ? 1.0f : __builtin_amdgcn_exp2f((l - mx) * c);
-    return (u64_t)(w * 17592186044416.0f);  // 2^44
-}
+// The exponent of a logit's weight; far below 0 for -inf and NaN, whose integer weight is 0.
+__device__ __forceinline__ float exponent(float l, float mx, float c) { return l == mx ? 0.0f : fmaxf((l - mx) * c, -200.0f); }
+__device__ __forceinline__ u64_t fixed(float y) { return (u64_t)(__builtin_amdgcn_exp2f(y) * 17592186044416.0f); }  // 2^44
+__device__ __forceinline__ u64_t weight_fix(float l, float mx, float c) { return fixed(exponent(l, mx, c)); }
 // kBins bins of equal width below the maximum, as far as the least logit or 24 temperatures (where a token's
 // weight is 2^-34 of the largest); what is below is in the last one.
 struct Bins {
-    float mx, inv;
-    __device__ Bins(float mx, float mn, float c) : mx(mx) {
-        const float span = fminf(mx - mn, 24.0f * (float)kLog2e64 / c);
-        inv = span > 0.0f && span < INFINITY ? (float)kBins / span : 0.0f;
+    float mx, c, per;  // per: bins for a step of -1 in the exponent
+    __device__ Bins(float mx, float mn, float c) : mx(mx), c(c) {
+        const float span = fminf((mx - mn) * c, 24.0f * (float)kLog2e64);
+        per = span > 0.0f ? -(float)kBins / span : 0.0f;
     }
-    __device__ int operator()(float l) const {
-        const float d = (mx - l) * inv;
-        return l == mx ? 0 : (d < (float)(kBins - 1) ? (int)d : kBins - 1);
-    }
+    __device__ int of(float y) const { return (int)fminf(y * per, (float)(kBins - 1)); }
+    __device__ int operator()(float l) const { return of(exponent(l, mx, c)); }
 };
 __device__ __forceinline__ void send(u64_t* p, u64_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ u64_t receive(const u64_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
@@ -403,7 +401,7 @@ __device__ __forceinline__ void find_bin(u64_t mass, u64_t before, u64_t target,
 
 constexpr int kCutEach = kCutChunk / kCutThreads;
 __global__ __launch_bounds__(kCutThreads) void k_ver_bins(const VerifyArgs a, const VerWork wk) {
-    __shared__ u64_t mass[kBins], red[(kCutThreads / kWave)];
+    __shared__ u64_t mass[kBins + 64], red[(kCutThreads / kWave)];  // the last 64: the last bin's, by lane
     __shared__ u64_t sh_before;
     __shared__ int sh, sh_bin;
     static_assert(kBins == kCutThreads, "a bin a thread");
@@ -411,24 +409,24 @@ __global__ __launch_bounds__(kCutThreads) void k_ver_bins(const VerifyArgs a, co
     float v[kCutEach];
     take<kCutEach, false>(a.logits + (int64_t)row * a.ld + x0, n, NAN, v);
     mass[tid] = 0;
+    if (tid < 64) mass[kBins + tid] = 0;
     float mx, mn;
     row_range(wk, row, mx, mn);
     __syncthreads();
     const float c = (float)(kLog2e64 / (double)a.temperature);
     const Bins bin(mx, mn, c);
-    u64_t low = 0;
+    // no branches: most logits are in the last bin, and go to a place of their lane's
 #pragma unroll
     for (int k = 0; k < kCutEach; ++k) {
-        if (!(v[k] <= mx)) continue;
-        const int b = bin(v[k]);
-        const u64_t w = weight_fix(v[k], mx, c);
-        if (b == kBins - 1)
-            low += w;
-        else
-            atomicAdd(&mass[b], w);
+        const float y = exponent(v[k], mx, c);
+        const int b = bin.of(y);
+        atomicAdd(&mass[b == kBins - 1 ? kBins + (tid & 63) : b], fixed(y));
     }
-    low = wave_fold(low, [](u64_t x, u64_t y) { return x + y; });
-    if ((tid & 63) == 0 && low) atomicAdd(&mass[kBins - 1], low);
+    __syncthreads();
+    if (tid < 64) {
+        const u64_t low = wave_fold(mass[kBins + tid], [](u64_t x, u64_t y) { return x + y; });
+        if (tid == 0) mass[kBins - 1] = low;
+    }
     __syncthreads();
     u64_t* part = wk.mass + (int64_t)row * wk.n_cuts * kBins;
     send(part + blockIdx.x * kBins + tid, mass[tid]);
@@ -496,8 +494,11 @@ __device__ void settle(Each each_of, u64_t before, u64_t target, float mx, float
         uint32_t a = 0xFFFFFFFFu, b = 0;
         each_of([&](int x, float l) {
             if (!inside(l)) return;
-            const uint32_t k = logit_key(l), at = atomicAdd(&s.n, 1u);
-            if (at < kFew) s.few[at] = make_uint2(__float_as_uint(l), (uint32_t)x);
+            const uint32_t k = logit_key(l);
+            if (*(volatile uint32_t*)&s.n <= kFew) {  // past that only how many keys there are matters
+                const uint32_t at = atomicAdd(&s.n, 1u);
+                if (at < kFew) s.few[at] = make_uint2(__float_as_uint(l), (uint32_t)x);
+            }
             a = min(a, k);
             b = max(b, k);
         });
