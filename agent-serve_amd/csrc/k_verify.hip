@@ -46,7 +46,9 @@ constexpr int kChunk = 4096;
 constexpr int kMaxChunks = (TF_HIP_VERIFY_MAX_VOCAB + kChunk - 1) / kChunk;
 // The nucleus' kernels: 16 logits a thread like the others, but half as many workgroups to count (a 64-node tree
 // over 128,256 logits: 256 threads 55.1 us a call, 512 54.2, 1024 60.8).
-constexpr int kCutThreads = 512, kCutChunk = 16 * kCutThreads, kBins = kCutThreads, kList = 4096, kFew = 256;
+constexpr int kCutThreads = 512, kCutChunk = 16 * kCutThreads, kBins = kCutThreads, kList = 4096, kFew = 64;
+constexpr int kBinBits = 9, kIndexBits = 19;
+static_assert(1 << kBinBits == kBins && 1 << kIndexBits == TF_HIP_VERIFY_MAX_VOCAB, "bits of a bin and of an index");
 constexpr double kLog2e64 = 1.4426950408889634;
 
 // Of one chunk of a row: its largest logit, that one's first index, and the weights' sum, the largest's 1.
@@ -465,7 +467,7 @@ __global__ __launch_bounds__(kCutThreads) void k_ver_bins(const VerifyArgs a, co
 // are ranked, or one logit many times over, of which the k-th in index order is the last.
 struct Settle {
     u64_t mass[kBins], red[(kCutThreads / kWave)];
-    uint2 few[kFew];
+    uint4 few[kFew];  // key, index, mass
     u64_t before;
     uint2 end;  // of the last token kept
     uint32_t n, k_lo, k_hi;
@@ -497,7 +499,8 @@ __device__ void settle(Each each_of, u64_t before, u64_t target, float mx, float
             const uint32_t k = logit_key(l);
             if (*(volatile uint32_t*)&s.n <= kFew) {  // past that only how many keys there are matters
                 const uint32_t at = atomicAdd(&s.n, 1u);
-                if (at < kFew) s.few[at] = make_uint2(__float_as_uint(l), (uint32_t)x);
+                const u64_t w = weight_fix(l, mx, c);
+                if (at < kFew) s.few[at] = make_uint4(k, (uint32_t)x, (uint32_t)w, (uint32_t)(w >> 32));
             }
             a = min(a, k);
             b = max(b, k);
@@ -527,32 +530,38 @@ __device__ void settle(Each each_of, u64_t before, u64_t target, float mx, float
         const uint32_t key = s.k_lo;
         const float l1 = __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
         const u64_t w = max(weight_fix(l1, mx, c), (u64_t)1), k = (target - before + w - 1) / w;
-        int a = 0, b = TF_HIP_VERIFY_MAX_VOCAB - 1;  // the least index with k of them up to it
-        while (a < b) {
-            const int mid = a + (b - a) / 2;
-            u64_t have = 0;
-            each_of([&](int x, float l) { have += x <= mid && logit_key(l) == key ? 1 : 0; });
-            have = block_fold(have, s.red, [](u64_t x, u64_t y) { return x + y; });
-            if (have >= k)
-                b = mid;
-            else
-                a = mid + 1;
+        // the index of the k-th: its bits from the highest on, kBins ranges of indices at a time
+        int first = 0;
+        u64_t have = 0;
+        for (int shift = kIndexBits; shift > 0;) {
+            const int above = shift;
+            shift = max(0, shift - kBinBits);
+            __syncthreads();
+            s.mass[tid] = 0;
+            __syncthreads();
+            each_of([&](int x, float l) {
+                if (logit_key(l) == key && x >> above == first >> above) atomicAdd(&s.mass[(x >> shift) & (kBins - 1)], (u64_t)1);
+            });
+            __syncthreads();
+            find_bin(s.mass[tid], have, k, s.red, &s.bin, &s.before);
+            have = s.before;
+            first |= s.bin << shift;
         }
+        const int a = first;
         thr = l1;
         cut = a;
         return;
     }
     __syncthreads();
     if (tid < m) {
-        const float l = __uint_as_float(s.few[tid].x);
-        const uint32_t k = logit_key(l), x = s.few[tid].y;
+        const uint4 me = s.few[tid];
         u64_t sum = before;
         for (int j = 0; j < m; ++j) {
-            const float lj = __uint_as_float(s.few[j].x);
-            const uint32_t kj = logit_key(lj);
-            if (kj > k || (kj == k && s.few[j].y < x)) sum += weight_fix(lj, mx, c);
+            const uint4 it = s.few[j];
+            if (it.x > me.x || (it.x == me.x && it.y < me.y)) sum += (u64_t)it.w << 32 | it.z;
         }
-        if (sum < target && sum + weight_fix(l, mx, c) >= target) s.end = s.few[tid];
+        if (sum < target && sum + ((u64_t)me.w << 32 | me.z) >= target)
+            s.end = make_uint2(me.x & 0x80000000u ? me.x & 0x7FFFFFFFu : ~me.x, me.y);
     }
     __syncthreads();
     thr = __uint_as_float(s.end.x);
