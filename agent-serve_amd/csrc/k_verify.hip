@@ -358,20 +358,28 @@ __device__ __forceinline__ void row_range(const VerWork& wk, int row, float& mx,
 // The sums that find where it ends are of 32-bit weights (the last token's place is off only where the
 // running sum comes within 1e-7 of top_p), as integers of 2^-44 of the largest: integers add up to the
 // same in any order, so the atomics do not show. What is kept is summed in 64 bits.
-// The exponent of a logit's weight; far below 0 for -inf and NaN, whose integer weight is 0.
-__device__ __forceinline__ float exponent(float l, float mx, float c) { return l == mx ? 0.0f : fmaxf((l - mx) * c, -200.0f); }
-__device__ __forceinline__ u64_t fixed(float y) { return (u64_t)(__builtin_amdgcn_exp2f(y) * 17592186044416.0f); }  // 2^44
-__device__ __forceinline__ u64_t weight_fix(float l, float mx, float c) { return fixed(exponent(l, mx, c)); }
+struct Weight32 {
+    float mx, c, rest;  // c + rest = log2(e) / T: c alone is up to 2^-25 off, the same way for every token
+    __device__ Weight32(float mx, double c64) : mx(mx), c((float)c64), rest(c < INFINITY ? (float)(c64 - (double)c) : 0.0f) {}
+    // far below 0 for -inf and NaN, whose integer weight is 0
+    __device__ float exponent(float l) const {
+        const float d = l - mx;
+        return l == mx ? 0.0f : fmaxf(fmaf(d, rest, d * c), -200.0f);
+    }
+    __device__ static u64_t fixed(float y) { return (u64_t)(__builtin_amdgcn_exp2f(y) * 17592186044416.0f); }  // 2^44
+    __device__ u64_t operator()(float l) const { return fixed(exponent(l)); }
+};
 // kBins bins of equal width below the maximum, as far as the least logit or 24 temperatures (where a token's
 // weight is 2^-34 of the largest); what is below is in the last one.
 struct Bins {
-    float mx, c, per;  // per: bins for a step of -1 in the exponent
-    __device__ Bins(float mx, float mn, float c) : mx(mx), c(c) {
-        const float span = fminf((mx - mn) * c, 24.0f * (float)kLog2e64);
+    Weight32 w;
+    float per;  // bins for a step of -1 in the exponent
+    __device__ Bins(const Weight32& w, float mn) : w(w) {
+        const float span = fminf((w.mx - mn) * w.c, 24.0f * (float)kLog2e64);
         per = span > 0.0f ? -(float)kBins / span : 0.0f;
     }
     __device__ int of(float y) const { return (int)fminf(y * per, (float)(kBins - 1)); }
-    __device__ int operator()(float l) const { return of(exponent(l, mx, c)); }
+    __device__ int operator()(float l) const { return of(w.exponent(l)); }
 };
 __device__ __forceinline__ void send(u64_t* p, u64_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ u64_t receive(const u64_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
@@ -415,14 +423,13 @@ __global__ __launch_bounds__(kCutThreads) void k_ver_bins(const VerifyArgs a, co
     float mx, mn;
     row_range(wk, row, mx, mn);
     __syncthreads();
-    const float c = (float)(kLog2e64 / (double)a.temperature);
-    const Bins bin(mx, mn, c);
+    const Bins bin(Weight32(mx, kLog2e64 / (double)a.temperature), mn);
     // no branches: most logits are in the last bin, and go to a place of their lane's
 #pragma unroll
     for (int k = 0; k < kCutEach; ++k) {
-        const float y = exponent(v[k], mx, c);
+        const float y = bin.w.exponent(v[k]);
         const int b = bin.of(y);
-        atomicAdd(&mass[b == kBins - 1 ? kBins + (tid & 63) : b], fixed(y));
+        atomicAdd(&mass[b == kBins - 1 ? kBins + (tid & 63) : b], Weight32::fixed(y));
     }
     __syncthreads();
     if (tid < 64) {
@@ -474,7 +481,7 @@ struct Settle {
     int bin;
 };
 template <class Each>
-__device__ void settle(Each each_of, u64_t before, u64_t target, float mx, float c, Settle& s, float& thr, int32_t& cut) {
+__device__ void settle(Each each_of, u64_t before, u64_t target, const Weight32& weight_of, Settle& s, float& thr, int32_t& cut) {
     const int tid = threadIdx.x;
     uint32_t lo = 0, hi = 0xFFFFFFFFu;
     auto inside = [&](float l) {
@@ -499,7 +506,7 @@ __device__ void settle(Each each_of, u64_t before, u64_t target, float mx, float
             const uint32_t k = logit_key(l);
             if (*(volatile uint32_t*)&s.n <= kFew) {  // past that only how many keys there are matters
                 const uint32_t at = atomicAdd(&s.n, 1u);
-                const u64_t w = weight_fix(l, mx, c);
+                const u64_t w = weight_of(l);
                 if (at < kFew) s.few[at] = make_uint4(k, (uint32_t)x, (uint32_t)w, (uint32_t)(w >> 32));
             }
             a = min(a, k);
@@ -516,7 +523,7 @@ __device__ void settle(Each each_of, u64_t before, u64_t target, float mx, float
         int shift = 0;
         while (((hi - lo) >> shift) >= (uint32_t)kBins) ++shift;
         each_of([&](int, float l) {
-            if (inside(l)) atomicAdd(&s.mass[(hi - logit_key(l)) >> shift], weight_fix(l, mx, c));
+            if (inside(l)) atomicAdd(&s.mass[(hi - logit_key(l)) >> shift], weight_of(l));
         });
         __syncthreads();
         find_bin(s.mass[tid], before, target, s.red, &s.bin, &s.before);
@@ -529,7 +536,7 @@ __device__ void settle(Each each_of, u64_t before, u64_t target, float mx, float
     if (m > kFew) {
         const uint32_t key = s.k_lo;
         const float l1 = __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
-        const u64_t w = max(weight_fix(l1, mx, c), (u64_t)1), k = (target - before + w - 1) / w;
+        const u64_t w = max(weight_of(l1), (u64_t)1), k = (target - before + w - 1) / w;
         // the index of the k-th: its bits from the highest on, kBins ranges of indices at a time
         int first = 0;
         u64_t have = 0;
@@ -581,8 +588,7 @@ __global__ __launch_bounds__(kCutThreads) void k_ver_cut(const VerifyArgs a, con
     const float mx = cut.mx;
     const int b0 = cut.bin;
     const double c64 = kLog2e64 / (double)a.temperature;
-    const float c = (float)c64;
-    const Bins bin(mx, cut.mn, c);
+    const Bins bin(Weight32(mx, c64), cut.mn);
     if (tid == 0) n_here = 0;
     __syncthreads();
     double above = 0.0;
@@ -613,7 +619,7 @@ __global__ __launch_bounds__(kCutThreads) void k_ver_cut(const VerifyArgs a, con
     z = block_sum(z, s.red);
     double in = 0.0;
     auto settle_of = [&](auto each_of) {
-        settle(each_of, cut.before, cut.target, mx, c, s, r.thr, r.cut);
+        settle(each_of, cut.before, cut.target, bin.w, s, r.thr, r.cut);
         each_of([&](int x, float l) {
             if (kept(r, l, x)) in += weight(l, mx, c64);
         });

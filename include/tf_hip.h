@@ -282,9 +282,9 @@ int tf_hip_attn_decode_noalloc(int device, const float* q, const float* k_cache,
  *
  * As tf_hip_attn_decode_noalloc: pointers are memory of `device` unless said otherwise, the
  * work is enqueued on `stream` (a hipStream_t of that device; NULL for the null stream) and
- * not waited for, and nothing is allocated, freed or synchronised; calls may be captured
- * into a graph once one has been made on the device outside capture (it loads the code). The
- * caller's current device is left as it was. Intermediate results live in the caller's workspace `ws` (16-byte aligned, ws_bytes >= what the _ws call says,
+ * not waited for, and nothing is allocated, freed or synchronised. A function's calls may be
+ * captured into a graph once it has been called on the device outside capture (that loads its
+ * code). The caller's current device is left as it was. Intermediate results live in the caller's workspace `ws` (16-byte aligned, ws_bytes >= what the _ws call says,
  * else TF_HIP_ESCRATCH), which belongs to the call until its work is done: calls that may
  * overlap, and graphs that may, take one each. Its contents need no initialisation. */
 #define TF_HIP_TREE_MAX 256

@@ -158,6 +158,21 @@ def test_attn_tree_masks(lib, n, mask, past, kv):
     Attn(8, 2, 64, n, past, mask=mask, kv=kv, seed=3).check(lib)
 
 
+@pytest.mark.parametrize("h,g,hd,n,past", [(1024, 4, 8, 3, 40), (1024, 1024, 8, 2, 10), (64, 1, 64, 256, 40),
+                                           (256, 1, 128, 5, 300)])
+def test_attn_tree_many_heads(lib, h, g, hd, n, past):
+    """Up to 1,024 query heads, over one kv head or as many: rows past one workgroup's, splits of one."""
+    Attn(h, g, hd, n, past, seed=16).check(lib)
+
+
+@pytest.mark.parametrize("kv", [F32, F16])
+@pytest.mark.parametrize("h,g,hd,n,past", [(8, 1, 64, 40, 16400), (6, 1, 128, 48, 16650), (9, 1, 72, 30, 17000)])
+def test_attn_tree_wide_workgroups(lib, h, g, hd, n, past, kv):
+    """Rows and steps enough for the workgroups of 256 rows, the last of them not full, the head size padded in
+    one."""
+    Attn(h, g, hd, n, past * 8, kv=kv, layout=n // 8 % 2, seed=17).check(lib)
+
+
 @pytest.mark.parametrize("pad,shift", [(0, 1), (5, 0), (64, 3)])
 @pytest.mark.parametrize("n", [1, 9, 70])
 def test_attn_tree_strides_and_alignment(lib, n, pad, shift):
@@ -402,6 +417,41 @@ def test_verify_tree_ties(lib, vocab, steps, top_p):
         x.logits = (np.floor(x.logits / 30 * steps) * (3.0 / steps)).astype(np.float32)
         if steps == 1:
             x.logits[:] = 2.5
+        x.check(lib)
+
+
+@pytest.mark.parametrize("sampled", [False, True])
+@pytest.mark.parametrize("top_p", [0.4, 1.0])
+@pytest.mark.parametrize("vocab", [1, 2, 3, 17])
+def test_verify_tree_small_vocabularies(lib, vocab, top_p, sampled):
+    """Down to one token, with more siblings than tokens."""
+    for seed in range(8):
+        Verify(9, vocab, 4, sampled, scale=1.0, top_p=top_p, seed=100 + seed).check(lib)
+
+
+@pytest.mark.parametrize("top_p", [0.2, 0.77, 0.999])
+def test_verify_tree_crowded_bins(lib, top_p):
+    """One far logit stretches the row's range, so that tens of thousands of others, all different, share a bin;
+    and rows whose nucleus ends in the last bin, 24 temperatures down and further."""
+    for seed in range(3):
+        x = Verify(4, 60001, 2, False, scale=0.001, temperature=0.9, top_p=top_p, seed=110 + seed)
+        x.logits[:, 7] = -15.0
+        x.logits[1] = np.where(np.arange(60001) == 99, 26.0, x.logits[1]).astype(np.float32)
+        x.check(lib)
+
+
+def test_verify_tree_many_rejections(lib):
+    """Nodes with up to 40 children sampled from a distribution far from the target's, so that most are rejected
+    and one sum over the row follows another."""
+    for seed in range(6):
+        x = Verify(60, 3001, 40, True, scale=2.0, top_p=(1.0, 0.9)[seed % 2], seed=120 + seed)
+        rng = np.random.default_rng(seed)
+        d = np.exp(2.0 * rng.standard_normal((60, 3001)))
+        x.draft = (d / d.sum(1, keepdims=True)).astype(np.float32)
+        for i in range(1, 60):
+            cum = np.cumsum(x.draft[x.parent[i]].astype(np.float64))
+            x.tokens[i] = min(int(np.searchsorted(cum, rng.random() * cum[-1])), 3000)
+        x.draws[1:] = 0.5 + 0.5 * x.draws[1:]
         x.check(lib)
 
 
