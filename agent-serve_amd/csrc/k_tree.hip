@@ -572,7 +572,7 @@ struct TreePlan {
     int hp, bm, blocks, splits;
 };
 
-TreePlan tree_plan(int n_tree, int H, int G, int hd, int n_past) {
+TreePlan tree_plan(int n_tree, int H, int G, int hd, int n_past, int size) {  // size: bytes of an element
     TreePlan p{};
     const int rows = n_tree * (H / G);
     p.hp = hd <= 64 ? 64 : (hd <= 128 ? 128 : 256);
@@ -585,7 +585,10 @@ TreePlan tree_plan(int n_tree, int H, int G, int hd, int n_past) {
     p.bm = big ? 256 : 64;
     p.blocks = (rows + p.bm - 1) / p.bm;
     const int64_t want = std::min(units, std::max<int64_t>(1, (big ? 256 : 512) / ((int64_t)G * p.blocks)));
-    const int64_t per = (units + want - 1) / want;
+    // Few steps run one after the other without a merge: they cost less than the second launch (1.3 us a step of fp32
+    // rows of 64, half that for fp16, 1.9 and 0.95 for rows of 128; the merge 3 us and its launch): 101 positions of 8
+    // fp32 heads of 64 take 9.0 us a call in one split and 11.0 in four, 161 take 11.9 and 10.9.
+    const int64_t per = units * p.hp * size <= 1024 ? units : (units + want - 1) / want;
     p.splits = (int)((units + per - 1) / per);
     return p;
 }
@@ -607,13 +610,13 @@ hipError_t launch_tree_type(const TreeAttnArgs& a, const TreePlan& p, hipStream_
 }  // namespace
 
 size_t tree_attn_ws_bytes(int n_tree, int H, int G, int hd, int n_past) {
-    const int S = tree_plan(n_tree, H, G, hd, n_past).splits;
+    const int S = std::max(tree_plan(n_tree, H, G, hd, n_past, 4).splits, tree_plan(n_tree, H, G, hd, n_past, 2).splits);
     return S == 1 ? 0 : (size_t)n_tree * H * S * (hd + 2) * 4;
 }
 
 hipError_t launch_tree_attn(const TreeAttnArgs& args, void* ws, hipStream_t st) {
     TreeAttnArgs a = args;
-    const TreePlan p = tree_plan(a.n_tree, a.H, a.G, a.hd, a.n_past);
+    const TreePlan p = tree_plan(a.n_tree, a.H, a.G, a.hd, a.n_past, a.kv_type == TF_HIP_TYPE_F32 ? 4 : 2);
     a.mask_words = (a.n_tree + 63) / 64;
     a.S = p.splits;
     a.part_o = (float*)ws;
