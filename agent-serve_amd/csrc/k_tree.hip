@@ -493,8 +493,7 @@ __global__ __launch_bounds__(64 * NW) void k_tree_attn(const TreeAttnArgs a) {
 
 // Merges the splits: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s (the weights are powers of two).
 // tpr threads a row, in groups of hd / 4: a thread takes 4 dims of every (tpr / (hd / 4))-th split in one
-// round of loads, and the groups meet in LDS. Bound by its launch and that round: 4 to 5 us for up to 10 MB of
-// partial rows, 11 us for 68 MB.
+// round of loads, and the groups meet in LDS. Bound by its launch and that round.
 __global__ __launch_bounds__(kBlock) void k_tree_merge(const TreeAttnArgs a, int tpr) {
     __shared__ f4_t part[kBlock];
     __shared__ float2 mls[kBlock];
@@ -633,8 +632,9 @@ hipError_t launch_tree_attn(const TreeAttnArgs& args, void* ws, hipStream_t st) 
     a.part_ml = a.part_o + (size_t)a.n_tree * a.H * a.S * a.hd;
     const hipError_t e = a.kv_type == TF_HIP_TYPE_F32 ? launch_tree_type<float>(a, p, st) : launch_tree_type<_Float16>(a, p, st);
     if (e != hipSuccess || a.S == 1) return e;
-    // up to 8 splits are one round for a wave; more are one for four waves (33 splits by one wave took 15 us, not 5)
-    const int tpr = a.S <= 8 ? 64 : kBlock, rows = a.n_tree * a.H, per = kBlock / tpr;
+    // a wave a row while that leaves a thread 16 splits, two rounds of loads, else four waves: a call over 8,191 fp16
+    // positions (16 splits of 64 dims) takes 25.2 us so and 27.7 by four, over 4,096 of 128 dims (65 splits) 21.4 and 18.9
+    const int tpr = a.S * (a.hd >> 2) <= 64 * 16 ? 64 : kBlock, rows = a.n_tree * a.H, per = kBlock / tpr;
     return launch_kernel(k_tree_merge, dim3((unsigned)((rows + per - 1) / per)), dim3(kBlock), st, a, tpr);
 }
 

@@ -274,19 +274,20 @@ int tf_hip_attn_decode_noalloc(int device, const float* q, const float* k_cache,
 /* ---------------------------------------------------------------- trees of drafted tokens
  * One step of speculative decoding over a device-resident cache. No counterpart in the
  * reference: they are for loops that draft several tokens, run the model once over all of
- * them and keep what it agrees with, with the same results as decoding them one by one
+ * them and keep what it agrees with: the tokens come out distributed as if decoded one by one
  * (attn_decode, attention.cpp:55-80; sample_logits, sampler.cpp:15-52). A tree has n_tree
  * nodes, at most TF_HIP_TREE_MAX; node 0 is the last token that is settled, and a node's
  * parent comes before it. Node i's key and value rows are at cache position n_past + i
- * (n_past + n_tree at most 2^30).
+ * (n_past + n_tree at most 2^30), rotated for its token's position, n_past plus its depth.
  *
  * As tf_hip_attn_decode_noalloc: pointers are memory of `device` unless said otherwise, the
  * work is enqueued on `stream` (a hipStream_t of that device; NULL for the null stream) and
  * not waited for, and nothing is allocated, freed or synchronised. A function's calls may be
  * captured into a graph once it has been called on the device outside capture (that loads its
- * code). The caller's current device is left as it was. Intermediate results live in the caller's workspace `ws` (16-byte aligned, ws_bytes >= what the _ws call says,
- * else TF_HIP_ESCRATCH), which belongs to the call until its work is done: calls that may
- * overlap, and graphs that may, take one each. Its contents need no initialisation. */
+ * code). The caller's current device is left as it was. Intermediate results live in the
+ * caller's workspace `ws` (16-byte aligned, ws_bytes >= what the _ws call says, else
+ * TF_HIP_ESCRATCH), which belongs to the call until its work is done: calls that may overlap,
+ * and graphs that may, take one each. Its contents need no initialisation. */
 #define TF_HIP_TREE_MAX 256
 
 /* Host only, no GPU: each node's own bit and its ancestors', from host parents (parent[0] < 0,
