@@ -33,12 +33,12 @@
 // that, and counts itself; the one that counts all takes them in the same way. No workgroup waits for another.
 //
 // What bounds them (128,256 logits a row unless said): k_ver_chunks for 64 rows the reading (33 MB in 9 to 10 us;
-// with the 64-bit sums the vector units, 17), for 5 its launch (5 us). k_ver_bins 14 us and k_ver_cut 17 for 64 rows,
-// half of either the way from the first workgroup's parts to the last one's result (11 and 10 for 26 rows of
-// 151,936); 4 of k_ver_cut's are its 64-bit masses. k_ver_walk 10 to 14 us, a chain of dependent rounds: nodes,
-// their logits, the rows, the sums, the drawn chunk (3 to 4 us of it the draw); 24 us more for each third or later
-// sibling tried, a whole row read by every workgroup. Whole calls: chain of 5 14.6 us, 64-node nucleus tree 52,
-// 6 sampled nodes over 151,936 19.5, 26 with a nucleus 46 to 70.
+// with the 64-bit sums the vector units, 17), for 5 its launch (5 us). k_ver_bins 14 us and k_ver_cut 13 for 64 rows,
+// half of either the way from the first workgroup's parts to the last one's result (11 and 9 for 26 rows of
+// 151,936). k_ver_walk 10 to 14 us, a chain of dependent rounds: nodes, their logits, the rows, the sums, the drawn
+// chunk (3 to 4 us of it the draw); 24 us more for each third or later sibling tried, a whole row read by every
+// workgroup. Whole calls: chain of 5 14.3 us, 64-node nucleus tree 47, 6 sampled nodes over 151,936 20, 26 with a
+// nucleus 46 to 73.
 #include <climits>
 
 #include "dev_common.hpp"
@@ -74,10 +74,10 @@ struct VerRow {
     int32_t cut;
     int32_t arg;
 };
-// A row on the way to its nucleus: its range, the bin of k_ver_bins that its end lies in, the mass below that bin,
-// and the counts of workgroups that are done and of listed tokens.
+// A row on the way to its nucleus: the bin of k_ver_bins that its end lies in, the mass above that bin, the
+// mass that the kept tokens reach, and the counts of workgroups that are done and of listed tokens.
 struct VerCut {
-    u64_t below;
+    u64_t before, target;
     float mx, mn;
     int32_t bin;
     uint32_t binned, listed, done;
@@ -363,17 +363,9 @@ __device__ __forceinline__ void row_range(const VerWork& wk, int row, float& mx,
 }
 
 // ---------------------------------------------------------------- the nucleus
-// k_ver_bins finds the bin that it ends in from 32-bit weights; within the bin the end is found from 64-bit ones,
-// the sum above the bin among them. The 32-bit weights have a say in the total by what is below the bin (1e-7 of
-// about 1 - top_p), and where the running sum meets top_p at the bin's edge (1e-7 of top_p, a token's place). Masses
-// are integers of 2^-44 of the largest weight: they add up to the same in any order, so the atomics do not show.
-constexpr double kMass = 17592186044416.0;  // 2^44
-// The mass that the kept tokens reach: a token is kept while the sum before it is below top_p.
-__device__ __forceinline__ u64_t mass_of(float top_p, u64_t all) {
-    const double want = (double)fmaxf(top_p, 0.0f) * (double)all;
-    const u64_t target = (u64_t)want;
-    return (double)target < want ? target + 1 : target;
-}
+// The sums that find where it ends are of 32-bit weights (the last token's place is off only where the
+// running sum comes within 1e-7 of top_p), as integers of 2^-44 of the largest: integers add up to the
+// same in any order, so the atomics do not show. What is kept is summed in 64 bits.
 struct Weight32 {
     float mx, c, rest;  // c + rest = log2(e) / T: c alone is up to 2^-25 off, the same way for every token
     __device__ Weight32(float mx, double c64) : mx(mx), c((float)c64), rest(c < INFINITY ? (float)(c64 - (double)c) : 0.0f) {}
@@ -382,7 +374,8 @@ struct Weight32 {
         const float d = l - mx;
         return l == mx ? 0.0f : fmaxf(fmaf(d, rest, d * c), -200.0f);
     }
-    __device__ static u64_t fixed(float y) { return (u64_t)(__builtin_amdgcn_exp2f(y) * (float)kMass); }
+    __device__ static u64_t fixed(float y) { return (u64_t)(__builtin_amdgcn_exp2f(y) * 17592186044416.0f); }  // 2^44
+    __device__ u64_t operator()(float l) const { return fixed(exponent(l)); }
 };
 // kBins bins of equal width below the maximum, as far as the least logit or 24 temperatures (where a token's
 // weight is 2^-34 of the largest); what is below is in the last one.
@@ -427,7 +420,7 @@ __device__ __forceinline__ void find_bin(u64_t mass, u64_t before, u64_t target,
 constexpr int kCutEach = kCutChunk / kCutThreads;
 __global__ __launch_bounds__(kCutThreads) void k_ver_bins(const VerifyArgs a, const VerWork wk) {
     __shared__ u64_t mass[kBins + 64], red[(kCutThreads / kWave)];  // the last 64: the last bin's, by lane
-    __shared__ u64_t sh_before, sh_in;
+    __shared__ u64_t sh_before;
     __shared__ int sh, sh_bin;
     static_assert(kBins == kCutThreads, "a bin a thread");
     const int tid = threadIdx.x, row = blockIdx.y, x0 = blockIdx.x * kCutChunk, n = min(kCutChunk, a.vocab - x0);
@@ -466,16 +459,18 @@ __global__ __launch_bounds__(kCutThreads) void k_ver_bins(const VerifyArgs a, co
         for (int j = 0; j < kRound; ++j) m += i + j < wk.n_cuts ? x[j] : 0;
     }
     const u64_t all = block_fold(m, red, [](u64_t x, u64_t y) { return x + y; });
-    const u64_t target = min(max(mass_of(a.top_p, all), (u64_t)1), max(all, (u64_t)1));
+    const double want = (double)fmaxf(a.top_p, 0.0f) * (double)all;
+    u64_t target = (u64_t)want;
+    if ((double)target < want) ++target;  // a token is kept while the sum before it is below top_p
+    target = target < 1 ? 1 : (target > all ? all : target);
     if (tid == 0) {
         sh_bin = 0;
-        sh_before = sh_in = 0;
+        sh_before = 0;
     }
     find_bin(m, 0, target, red, &sh_bin, &sh_before);
-    if (tid == sh_bin) sh_in = m;
-    __syncthreads();
     if (tid == 0) {
-        cut.below = all - sh_before - sh_in;
+        cut.before = sh_before;
+        cut.target = target;
         cut.mx = mx;
         cut.mn = mn;
         cut.bin = sh_bin;
@@ -483,8 +478,8 @@ __global__ __launch_bounds__(kCutThreads) void k_ver_bins(const VerifyArgs a, co
 }
 
 // Which of a set of tokens the running sum ends at: `each` calls f(index, logit) for all of them (over the
-// workgroup's threads), weight_of gives their masses, `before` is the mass above them. Narrows their keys by bins
-// until few are left, which are ranked, or one logit many times over, of which the k-th in index order is the last.
+// workgroup's threads), `before` is the mass above them. Narrows their keys by bins until few are left, which
+// are ranked, or one logit many times over, of which the k-th in index order is the last.
 struct Settle {
     u64_t mass[kBins], red[(kCutThreads / kWave)];
     uint4 few[kFew];  // key, index, mass
@@ -493,8 +488,8 @@ struct Settle {
     uint32_t n, k_lo, k_hi;
     int bin;
 };
-template <class Each, class W>
-__device__ void settle(Each each_of, u64_t before, u64_t target, W weight_of, Settle& s, float& thr, int32_t& cut) {
+template <class Each>
+__device__ void settle(Each each_of, u64_t before, u64_t target, const Weight32& weight_of, Settle& s, float& thr, int32_t& cut) {
     const int tid = threadIdx.x;
     uint32_t lo = 0, hi = 0xFFFFFFFFu;
     auto inside = [&](float l) {
@@ -549,7 +544,7 @@ __device__ void settle(Each each_of, u64_t before, u64_t target, W weight_of, Se
     if (m > kFew) {
         const uint32_t key = s.k_lo;
         const float l1 = __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
-        const u64_t w = weight_of(l1), k = (target - before + w - 1) / w;
+        const u64_t w = max(weight_of(l1), (u64_t)1), k = (target - before + w - 1) / w;
         // the index of the k-th: its bits from the highest on, kBins ranges of indices at a time
         int first = 0;
         u64_t have = 0;
@@ -632,13 +627,7 @@ __global__ __launch_bounds__(kCutThreads) void k_ver_cut(const VerifyArgs a, con
     z = block_sum(z, s.red);
     double in = 0.0;
     auto settle_of = [&](auto each_of) {
-        auto mass = [&](float l) { return max((u64_t)(weight(l, mx, c64) * kMass), (u64_t)1); };
-        u64_t inside = 0;
-        each_of([&](int, float l) { inside += mass(l); });
-        inside = block_fold(inside, s.red, [](u64_t x, u64_t y) { return x + y; });
-        // (k_ver_bins' choice of the bin stands where the sums differ by a token at its edge)
-        const u64_t before = (u64_t)(z * kMass), target = mass_of(a.top_p, before + inside + cut.below);
-        settle(each_of, before, min(max(target, before + 1), before + inside), mass, s, r.thr, r.cut);
+        settle(each_of, cut.before, cut.target, bin.w, s, r.thr, r.cut);
         each_of([&](int x, float l) {
             if (kept(r, l, x)) in += weight(l, mx, c64);
         });
