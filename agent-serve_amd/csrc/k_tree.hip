@@ -25,10 +25,10 @@
 //
 // What bounds it. Few positions: the launch and three dependent memory rounds (one query over 7 positions,
 // 5.2 us of kernel). A middling call: the same and the merge's launch (8 queries of 32 heads over 1,000 fp32
-// positions 6.4 + 4 us; 37 of 14 heads over 2,029 10.3 + 5). Many rows over long caches: the matrix pipes
+// positions 6 + 4 us; 37 of 14 heads over 2,029 10.3 + 4.5). Many rows over long caches: the matrix pipes
 // and, beside them, the softmax and the splitting of numbers (64 queries of 64 heads of 128 over 32,768 fp16
-// positions 145 us of kernel: 138 GFLOP of matrix work at 950 TFLOP/s, a large library product reaching
-// 1,205; the matrix pipes are busy 38 % of the cycles, the vector units 33 %).
+// positions 149 us, the merge's 8 among them: 138 GFLOP of matrix work at 980 TFLOP/s, a large library product
+// reaching 1,205; the matrix pipes are busy 38 % of the cycles, the vector units 33 %).
 #include <algorithm>
 #include <type_traits>
 
@@ -442,7 +442,7 @@ __global__ __launch_bounds__(64 * NW) void k_tree_attn(const TreeAttnArgs a) {
     barrier();
     // step t: its record is complete, the loads of t + 1 are there or under way. The next step's stores go first:
     // the waves leave the barrier together, and those on the vector units keep out of the way of the matrix ones
-    // (after the record 30.0 us instead of 27.7 for 64 queries of 32 heads over 8,191 fp16 positions).
+    // (after the record 2.3 us more, of 25.3, for 64 queries of 32 heads over 8,191 fp16 positions).
     auto step = [&](auto TREE, int t) __attribute__((always_inline)) {
         if (t + 1 < steps) store(t + 1);
         if (tid == 0) bad[(t + 2) % 3] = 0;
@@ -553,7 +553,7 @@ __global__ __launch_bounds__(kBlock) void k_tree_merge(const TreeAttnArgs a, int
 // up to the first entry that does not name a node past the one before. A thread owns 16 bytes of a row's
 // place and walks the path in order: path[i] >= i, so a row is read before an earlier entry's write could
 // reach it (that entry wrote a lower row). Bound by its launch and one dependent round a moved row: 3.5 us for 4
-// rows of 16 layers, 5.2 for 9 of 28 (1 MB read and written); a whole call is 7.4 us, the host's launch.
+// rows of 16 layers, 5.2 for 9 of 28 (1 MB read and written); a whole call is 7.9 us, the host's launch.
 __global__ __launch_bounds__(kBlock) void k_keep_path(const KeepArgs a) {
     const int64_t per_layer = (int64_t)a.G * a.row16;  // 16-byte pieces of one position
     const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
@@ -586,9 +586,9 @@ TreePlan tree_plan(int n_tree, int H, int G, int hd, int n_past, int size) {  //
     const int rows = n_tree * (H / G);
     p.hp = hd <= 64 ? 64 : (hd <= 128 ? 128 : 256);
     // Workgroups of 256 rows (head sizes up to 128) read keys and values fewest times and run two row subtiles on
-    // every fragment, but fill the chip only where there is enough (more than 128 rows): 16 steps for each of 256 workgroups. Below that,
-    // 64 rows and about two workgroups a CU. (64 queries of 64 heads of 128 over 32,768 fp16 positions: 178 us, by
-    // 64 rows 213; of 32 heads of 64 over 8,191: 31.0 and 29.3.)
+    // every fragment, but fill the chip only where there is enough (more than 128 rows): 16 steps for each of 256
+    // workgroups. Below that, 64 rows and about two workgroups a CU. (With an earlier merge, 64 queries of 64 heads of 128 over 32,768 fp16
+    // positions took 178 us, by 64 rows 213; of 32 heads of 64 over 8,191 31.0 and 29.3.)
     const int64_t units = ((int64_t)n_past + n_tree + kRec - 1) / kRec;
     const bool big = p.hp <= 128 && rows > 128 && (int64_t)G * ((rows + 255) / 256) * units >= 16 * 256;
     p.bm = big ? 256 : 64;
@@ -633,7 +633,7 @@ hipError_t launch_tree_attn(const TreeAttnArgs& args, void* ws, hipStream_t st) 
     const hipError_t e = a.kv_type == TF_HIP_TYPE_F32 ? launch_tree_type<float>(a, p, st) : launch_tree_type<_Float16>(a, p, st);
     if (e != hipSuccess || a.S == 1) return e;
     // a wave a row while that leaves a thread 16 splits, two rounds of loads, else four waves: a call over 8,191 fp16
-    // positions (16 splits of 64 dims) takes 25.2 us so and 27.7 by four, over 4,096 of 128 dims (65 splits) 21.4 and 18.9
+    // positions (16 splits of 64 dims) takes 25.3 us so and 27.7 by four, over 4,096 of 128 dims (65 splits) 21.4 and 18.9
     const int tpr = a.S * (a.hd >> 2) <= 64 * 16 ? 64 : kBlock, rows = a.n_tree * a.H, per = kBlock / tpr;
     return launch_kernel(k_tree_merge, dim3((unsigned)((rows + per - 1) / per)), dim3(kBlock), st, a, tpr);
 }

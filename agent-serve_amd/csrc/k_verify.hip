@@ -37,8 +37,8 @@
 // half of either the way from the first workgroup's parts to the last one's result (11 and 9 for 26 rows of
 // 151,936). k_ver_walk 10 to 14 us, a chain of dependent rounds: nodes, their logits, the rows, the sums, the drawn
 // chunk (3 to 4 us of it the draw); 24 us more for each third or later sibling tried, a whole row read by every
-// workgroup. Whole calls: chain of 5 14.3 us, 64-node nucleus tree 47, 6 sampled nodes over 151,936 20, 26 with a
-// nucleus 46 to 73.
+// workgroup. Whole calls: chain of 5 14.6 us, 64-node nucleus tree 49, 6 sampled nodes over 151,936 19.5, 26 with
+// a nucleus 46 to 70.
 #include <climits>
 
 #include "dev_common.hpp"
@@ -363,9 +363,12 @@ __device__ __forceinline__ void row_range(const VerWork& wk, int row, float& mx,
 }
 
 // ---------------------------------------------------------------- the nucleus
-// The sums that find where it ends are of 32-bit weights (the last token's place is off only where the
-// running sum comes within 1e-7 of top_p), as integers of 2^-44 of the largest: integers add up to the
-// same in any order, so the atomics do not show. What is kept is summed in 64 bits.
+// The sums that find where it ends are of 32-bit weights, as integers of 2^-44 of the largest: integers add up
+// to the same in any order, so the atomics do not show. A weight 2^-y is up to (2 y + 2) 2^-24 of itself off (its
+// exponent's three roundings and exp2's), so the end may be another token where the running sum comes within
+// 6e-7 of top_p (that far for one logit above half a million equal ones; 5e-10 in the one row of half a million
+// random ones where it showed). 64-bit weights in the bin that the end lies in leave the part below it as it is
+// and take 4 us more for 64 rows. What is kept is summed in 64 bits.
 struct Weight32 {
     float mx, c, rest;  // c + rest = log2(e) / T: c alone is up to 2^-25 off, the same way for every token
     __device__ Weight32(float mx, double c64) : mx(mx), c((float)c64), rest(c < INFINITY ? (float)(c64 - (double)c) : 0.0f) {}

@@ -317,8 +317,9 @@ int tf_hip_attn_tree(int device, int kv_type, const float* q, int64_t ldq, const
  * not looked at; a node whose parent does not come before it, or whose token is not below
  * n_vocab, is never accepted). The target's distribution P_i is softmax(logits / temperature)
  * cut to the nucleus of top_p as sample_logits cuts it, logits that compare equal in ascending
- * index order; temperature <= 0 is all on the first maximum. From node 0 on, a node's children
- * are tried in index order, child c against draws[c] (a uniform draw in [0, 1)):
+ * index order (where the running sum comes within 6e-7 of top_p, its end may be another token);
+ * temperature <= 0 is all on the first maximum. From node 0 on, a node's children are tried in
+ * index order, child c against draws[c] (a uniform draw in [0, 1)):
  *   draft NULL: the children are the drafter's choices; c is accepted with the probability P
  *     gives its token, of what earlier rejected tokens leave;
  *   draft: row i (of ld_draft floats) is the distribution that node i's children were sampled
@@ -341,8 +342,8 @@ int tf_hip_verify_tree(int device, const float* logits, int64_t ld_logits, int32
 /* Keeps the accepted nodes: in every layer's K and V cache (n_layer caches of n_kv max_seq hd
  * elements one after the other, as tf_hip_create lays them out; kv_type and layout as above)
  * the row of position n_past + path[i] moves to n_past + i for i < *n_path. The path's nodes
- * ascend, as tf_hip_verify_tree writes them (path and result): at the first that does not, or is not below
- * n_tree, the path ends. The other rows stay as they are. */
+ * ascend, as tf_hip_verify_tree writes them (path and result): at the first that does not, or is
+ * not below n_tree, the path ends. The other rows stay as they are. */
 int tf_hip_keep_path(int device, int kv_type, void* k_cache, void* v_cache, int32_t n_layer, int32_t n_kv, int32_t hd,
                      int32_t n_past, int32_t n_tree, int32_t max_seq, int32_t layout, const int32_t* path,
                      const int32_t* n_path, void* stream);
