@@ -102,8 +102,12 @@ __global__ __launch_bounds__(64 * NW) void k_tree_attn(const TreeAttnArgs a) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, gq = lane >> 4;
     const int hd = EXACT ? HP : a.hd, rep = a.H / a.G, rows = a.n_tree * rep;
-    // kv head fastest, then split, then row block: the row blocks of one span of keys are G S apart
-    const int g = blockIdx.x % a.G, split = blockIdx.x / a.G % a.S, blk = blockIdx.x / (a.G * a.S);
+    // A span of keys is a kv head's split (kv head fastest). Workgroups go to the 8 XCDs in turn: a span's row blocks
+    // are 8 apart, so that they meet in one XCD's L2, with spans rounded up to 8 of them.
+    const int blocks = (rows + 16 * QS * NW - 1) / (16 * QS * NW);
+    const int span = blockIdx.x / (8 * blocks) * 8 + blockIdx.x % 8, blk = blockIdx.x / 8 % blocks;
+    if (span >= a.G * a.S) return;
+    const int g = span % a.G, split = span / a.G;
     const int end = a.n_past + a.n_tree;
     const int units = (end + kRec - 1) / kRec, per = (units + a.S - 1) / a.S;
     const int u0 = split * per, steps = min(units - u0, per);
@@ -587,8 +591,8 @@ TreePlan tree_plan(int n_tree, int H, int G, int hd, int n_past, int size) {  //
     p.hp = hd <= 64 ? 64 : (hd <= 128 ? 128 : 256);
     // Workgroups of 256 rows (head sizes up to 128) read keys and values fewest times and run two row subtiles on
     // every fragment, but fill the chip only where there is enough (more than 128 rows): 16 steps for each of 256
-    // workgroups. Below that, 64 rows and about two workgroups a CU. (With an earlier merge, 64 queries of 64 heads of 128 over 32,768 fp16
-    // positions took 178 us, by 64 rows 213; of 32 heads of 64 over 8,191 31.0 and 29.3.)
+    // workgroups. Below that, 64 rows and about two workgroups a CU. (With an earlier merge, 64 queries of 64 heads
+    // of 128 over 32,768 fp16 positions took 178 us, by 64 rows 213; of 32 heads of 64 over 8,191 31.0 and 29.3.)
     const int64_t units = ((int64_t)n_past + n_tree + kRec - 1) / kRec;
     const bool big = p.hp <= 128 && rows > 128 && (int64_t)G * ((rows + 255) / 256) * units >= 16 * 256;
     p.bm = big ? 256 : 64;
@@ -605,7 +609,8 @@ TreePlan tree_plan(int n_tree, int H, int G, int hd, int n_past, int size) {  //
 template <class T, int HP, int NW, int QS>
 hipError_t launch_tree(const TreeAttnArgs& a, const TreePlan& p, hipStream_t st) {
     static_assert(HP == 256 || NW * QS == 4 || NW * QS == 16, "the plan's rows");
-    const dim3 grid((unsigned)(a.G * p.splits * p.blocks)), block(64 * NW);
+    const int spans = a.G * p.splits;
+    const dim3 grid((unsigned)(p.blocks == 1 ? spans : (spans + 7) / 8 * 8 * p.blocks)), block(64 * NW);
     return launch_kernel(a.hd == HP ? k_tree_attn<T, HP, NW, QS, true> : k_tree_attn<T, HP, NW, QS, false>, grid, block, st, a);
 }
 
