@@ -360,7 +360,7 @@ struct TreeAttnArgs {
     int64_t ldo;
     int kv_type, n_tree, H, G, hd, n_past, max_seq, layout;
     // set by launch_tree_attn
-    int mask_words, S;
+    int mask_words, S, group;
     float* part_o;   // [n_tree H][S][hd]
     float* part_ml;  // [n_tree H][S][2]
 };
