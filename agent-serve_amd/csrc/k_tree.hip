@@ -27,7 +27,7 @@
 // 5.2 us of kernel). A middling call: the same and the merge's launch (8 queries of 32 heads over 1,000 fp32
 // positions 6 + 4 us; 37 of 14 heads over 2,029 10.3 + 4.5). Many rows over long caches: the matrix pipes
 // and, beside them, the softmax and the splitting of numbers (64 queries of 64 heads of 128 over 32,768 fp16
-// positions 149 us, the merge's 8 among them: 138 GFLOP of matrix work at 980 TFLOP/s, a large library product
+// positions 146 us, the merge's 8 among them: 138 GFLOP of matrix work at 1,000 TFLOP/s, a large library product
 // reaching 1,205; the matrix pipes are busy 38 % of the cycles; 46 % issue to them or the vector units).
 #include <algorithm>
 #include <type_traits>
