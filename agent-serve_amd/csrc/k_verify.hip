@@ -33,12 +33,12 @@
 // that, and counts itself; the one that counts all takes them in the same way. No workgroup waits for another.
 //
 // What bounds them (128,256 logits a row unless said): k_ver_chunks for 64 rows the reading (33 MB in 9 to 10 us;
-// with the 64-bit sums the vector units, 17), for 5 its launch (5 us). k_ver_bins 14 us and k_ver_cut 13 for 64 rows,
-// half of either the way from the first workgroup's parts to the last one's result (11 and 9 for 26 rows of
+// with the 64-bit sums the vector units, 17), for 5 its launch (5 us). k_ver_bins 18 us and k_ver_cut 15 for 64 rows,
+// half of either the way from the first workgroup's parts to the last one's result (13 and 9 for 26 rows of
 // 151,936). k_ver_walk 10 to 14 us, a chain of dependent rounds: nodes, their logits, the rows, the sums, the drawn
 // chunk (3 to 4 us of it the draw); 24 us more for each third or later sibling tried, a whole row read by every
-// workgroup. Whole calls: chain of 5 14.6 us, 64-node nucleus tree 49, 6 sampled nodes over 151,936 19.5, 26 with
-// a nucleus 46 to 70.
+// workgroup. Whole calls: chain of 5 14.6 us, 64-node nucleus tree 55, 6 sampled nodes over 151,936 19.5, 26 with
+// a nucleus 48 to 72.
 #include <climits>
 
 #include "dev_common.hpp"
@@ -363,34 +363,41 @@ __device__ __forceinline__ void row_range(const VerWork& wk, int row, float& mx,
 }
 
 // ---------------------------------------------------------------- the nucleus
-// The sums that find where it ends are of 32-bit weights, as integers of 2^-44 of the largest: integers add up
-// to the same in any order, so the atomics do not show. A weight 2^-y is up to (2 y + 2) 2^-24 of itself off (its
-// exponent's three roundings and exp2's), so the end may be another token where the running sum comes within
-// 6e-7 of top_p (that far for one logit above half a million equal ones; 5e-10 in the one row of half a million
-// random ones where it showed). 64-bit weights in the bin that the end lies in leave the part below it as it is
-// and take 4 us more for 64 rows. What is kept is summed in 64 bits.
-struct Weight32 {
-    float mx, c, rest;  // c + rest = log2(e) / T: c alone is up to 2^-25 off, the same way for every token
-    __device__ Weight32(float mx, double c64) : mx(mx), c((float)c64), rest(c < INFINITY ? (float)(c64 - (double)c) : 0.0f) {}
-    // far below 0 for -inf and NaN, whose integer weight is 0
-    __device__ float exponent(float l) const {
-        const float d = l - mx;
-        return l == mx ? 0.0f : fmaxf(fmaf(d, rest, d * c), -200.0f);
+// The sums that find where it ends are of 64-bit weights as integers of 2^-44 of the largest: integers add up to
+// the same in any order, so the atomics do not show. Their roundings come to 2e-8 of the total at the very most
+// (half a million equal logits far below one), commonly 1e-11. 32-bit weights were 1e-9 off as a rule, which kept
+// another last token in one row of some 100,000 random ones, for 49.7 us instead of 55.2 with 64 rows of 128,256.
+struct Mass {
+    double mx, c;  // c = log2(e) / T
+    __device__ Mass(float mx, double c) : mx((double)mx), c(c) {}
+    // 2^(y + 44), rounded; 0 for -inf and NaN. 2^f is the Taylor series of e^(f ln 2) to its 9th power (|f| <= 1/2:
+    // the rest is below 7e-12 of it). What is added to 2^52 lies in the sum's low 52 bits.
+    __device__ u64_t operator()(float l) const {
+        const double y = (double)l == mx ? 0.0 : fmax(((double)l - mx) * c, -200.0), n = rint(y), f = y - n;
+        double p = 1.0178086009239699e-07;
+        p = fma(p, f, 1.3215486790144307e-06);
+        p = fma(p, f, 1.5252733804059841e-05);
+        p = fma(p, f, 1.5403530393381608e-04);
+        p = fma(p, f, 1.3333558146428443e-03);
+        p = fma(p, f, 9.6181291076284772e-03);
+        p = fma(p, f, 5.5504108664821580e-02);
+        p = fma(p, f, 2.4022650695910071e-01);
+        p = fma(p, f, 6.9314718055994531e-01);
+        p = fma(p, f, 1.0);
+        p = __builtin_amdgcn_ldexp(p, (int)n + 44) + 0x1p52;
+        return (u64_t)__double_as_longlong(p) & 0xFFFFFFFFFFFFFull;
     }
-    __device__ static u64_t fixed(float y) { return (u64_t)(__builtin_amdgcn_exp2f(y) * 17592186044416.0f); }  // 2^44
-    __device__ u64_t operator()(float l) const { return fixed(exponent(l)); }
 };
 // kBins bins of equal width below the maximum, as far as the least logit or 24 temperatures (where a token's
 // weight is 2^-34 of the largest); what is below is in the last one.
 struct Bins {
-    Weight32 w;
-    float per;  // bins for a step of -1 in the exponent
-    __device__ Bins(const Weight32& w, float mn) : w(w) {
-        const float span = fminf((w.mx - mn) * w.c, 24.0f * (float)kLog2e64);
-        per = span > 0.0f ? -(float)kBins / span : 0.0f;
+    float mx, scale;  // bins for a step of 1 in the logit: 32 bits do, as the roundings keep the logits' order
+    __device__ Bins(float mx, float mn, double c) : mx(mx) {
+        const float span = fminf((mx - mn) * (float)c, 24.0f * (float)kLog2e64);
+        scale = span > 0.0f ? (float)c * (-(float)kBins / span) : 0.0f;
     }
-    __device__ int of(float y) const { return (int)fminf(y * per, (float)(kBins - 1)); }
-    __device__ int operator()(float l) const { return of(w.exponent(l)); }
+    // -inf and NaN are in the last one
+    __device__ int operator()(float l) const { return l == mx ? 0 : (int)fminf((l - mx) * scale, (float)(kBins - 1)); }
 };
 __device__ __forceinline__ void send(u64_t* p, u64_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ u64_t receive(const u64_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
@@ -434,13 +441,14 @@ __global__ __launch_bounds__(kCutThreads) void k_ver_bins(const VerifyArgs a, co
     float mx, mn;
     row_range(wk, row, mx, mn);
     __syncthreads();
-    const Bins bin(Weight32(mx, kLog2e64 / (double)a.temperature), mn);
+    const double c = kLog2e64 / (double)a.temperature;
+    const Bins bin(mx, mn, c);
+    const Mass mass_of(mx, c);
     // no branches: most logits are in the last bin, and go to a place of their lane's
 #pragma unroll
     for (int k = 0; k < kCutEach; ++k) {
-        const float y = bin.w.exponent(v[k]);
-        const int b = bin.of(y);
-        atomicAdd(&mass[b == kBins - 1 ? kBins + (tid & 63) : b], Weight32::fixed(y));
+        const int b = bin(v[k]);
+        atomicAdd(&mass[b == kBins - 1 ? kBins + (tid & 63) : b], mass_of(v[k]));
     }
     __syncthreads();
     if (tid < 64) {
@@ -492,7 +500,7 @@ struct Settle {
     int bin;
 };
 template <class Each>
-__device__ void settle(Each each_of, u64_t before, u64_t target, const Weight32& weight_of, Settle& s, float& thr, int32_t& cut) {
+__device__ void settle(Each each_of, u64_t before, u64_t target, const Mass& weight_of, Settle& s, float& thr, int32_t& cut) {
     const int tid = threadIdx.x;
     uint32_t lo = 0, hi = 0xFFFFFFFFu;
     auto inside = [&](float l) {
@@ -599,7 +607,7 @@ __global__ __launch_bounds__(kCutThreads) void k_ver_cut(const VerifyArgs a, con
     const float mx = cut.mx;
     const int b0 = cut.bin;
     const double c64 = kLog2e64 / (double)a.temperature;
-    const Bins bin(Weight32(mx, c64), cut.mn);
+    const Bins bin(mx, cut.mn, c64);
     if (tid == 0) n_here = 0;
     __syncthreads();
     double above = 0.0;
@@ -630,7 +638,7 @@ __global__ __launch_bounds__(kCutThreads) void k_ver_cut(const VerifyArgs a, con
     z = block_sum(z, s.red);
     double in = 0.0;
     auto settle_of = [&](auto each_of) {
-        settle(each_of, cut.before, cut.target, bin.w, s, r.thr, r.cut);
+        settle(each_of, cut.before, cut.target, Mass(mx, c64), s, r.thr, r.cut);
         each_of([&](int x, float l) {
             if (kept(r, l, x)) in += weight(l, mx, c64);
         });

@@ -317,7 +317,7 @@ int tf_hip_attn_tree(int device, int kv_type, const float* q, int64_t ldq, const
  * not looked at; a node whose parent does not come before it, or whose token is not below
  * n_vocab, is never accepted). The target's distribution P_i is softmax(logits / temperature)
  * cut to the nucleus of top_p as sample_logits cuts it, logits that compare equal in ascending
- * index order (where the running sum comes within 6e-7 of top_p, its end may be another token);
+ * index order (where the running sum comes within 2e-8 of top_p, its end may be another token);
  * temperature <= 0 is all on the first maximum. From node 0 on, a node's children are tried in
  * index order, child c against draws[c] (a uniform draw in [0, 1)):
  *   draft NULL: the children are the drafter's choices; c is accepted with the probability P

@@ -440,6 +440,14 @@ def test_verify_tree_crowded_bins(lib, top_p):
         x.check(lib)
 
 
+@pytest.mark.parametrize("n,vocab,kw", [
+    (64, 4097, dict(seed=8001, width=2, scale=3.0, temperature=2.0, top_p=0.99, pad=5, shift=3)),
+    (16, 8192, dict(seed=1497, width=2, sampled=True, scale=1.0, temperature=1.0, top_p=0.5, pad=1))])
+def test_verify_tree_nucleus_border(lib, n, vocab, kw):
+    """A row's running sum passes top_p by 5e-10 and 4e-9: sums of 32-bit weights keep another last token."""
+    Verify(n, vocab, **kw).check(lib)
+
+
 def test_verify_tree_many_rejections(lib):
     """Nodes with up to 40 children sampled from a distribution far from the target's, so that most are rejected
     and one sum over the row follows another."""
